@@ -108,6 +108,20 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.fbmoe_forward_ep_dispatch.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, f32, i32, i32, vp, vp, u32,
                                                   vp, vp, sz, vp]
         lib.fbmoe_forward_ep_dispatch.restype = i32
+        i64 = ctypes.c_int64
+        lib.fbmoe_w4_bytes.argtypes = [i64, i32, i32, i32]
+        lib.fbmoe_w4_bytes.restype = sz
+        lib.fbmoe_quantize_w4.argtypes = [vp, i32, vp, vp, i64, i32, i32, i32, vp, vp]
+        lib.fbmoe_quantize_w4.restype = i32
+        lib.fbmoe_dequantize_w4.argtypes = [vp, i64, i32, i32, i32, i32, vp, vp]
+        lib.fbmoe_dequantize_w4.restype = i32
+        lib.fbmoe_linear_w4.argtypes = [vp, i64, i32, i32, vp, i32, i32, i32, vp, i64, vp]
+        lib.fbmoe_linear_w4.restype = i32
+        lib.fbmoe_w4_workspace_size.argtypes = [i32, i32, i32]
+        lib.fbmoe_w4_workspace_size.restype = sz
+        lib.fbmoe_forward_w4.argtypes = [vp, vp, vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, vp, vp, sz,
+                                         vp]
+        lib.fbmoe_forward_w4.restype = i32
         lib.fbmoe_ipc_alloc.argtypes = [sz, ctypes.POINTER(vp)]
         lib.fbmoe_ipc_alloc.restype = i32
         lib.fbmoe_ipc_free.argtypes = [vp]
@@ -433,6 +447,154 @@ def read_status(workspace: torch.Tensor) -> int:
     if rc not in (0, -6):
         _check(rc)
     return int(st.value)
+
+
+# ---------------------------------------------------------------- 4-bit weights with group scales
+# A packed matrix is a uint8 tensor [..., ceil(N / 16), K / 128, tile] (format: include/fbmoe.h); the tile's bytes tell
+# the group size.  These run on the tensors' own device and that device's current stream, and record no gradient.
+W4_MAX_TOKENS = 64
+_W4_GROUPS = {1024 + 4096 // g: g for g in (32, 64, 128)}
+_W4_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
+
+
+def _launch_on(dev: torch.device, fn, *args) -> None:
+    """Call a C entry point, its stream appended, with `dev` current."""
+    if dev.index == torch.cuda.current_device():
+        _check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            _check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _w4_shape(packed: torch.Tensor, name: str, n: int = None) -> Tuple[int, int, int]:
+    """(N, K, group) of a packed tensor; n: the rows in use, all of the tiles' by default."""
+    _require(isinstance(packed, torch.Tensor) and packed.dtype == torch.uint8 and packed.dim() >= 3
+             and packed.is_contiguous() and packed.size(-1) in _W4_GROUPS and packed.size(-2) > 0
+             and packed.size(-3) > 0,
+             f"{name} must be a contiguous uint8 tensor [..., ceil(N / 16), K / 128, tile] as quantize_w4 packs it")
+    rows = packed.size(-3) * 16
+    n = rows if n is None else int(n)
+    _require(rows - 16 < n <= rows, f"n must be in {rows - 15}..{rows} for {name}'s {packed.size(-3)} row tiles")
+    return n, packed.size(-2) * 128, _W4_GROUPS[packed.size(-1)]
+
+
+def quantize_w4(w: torch.Tensor, group_size: int = 128, scale: torch.Tensor = None,
+                block_scale: torch.Tensor = None) -> torch.Tensor:
+    """Weights [..., N, K] -> packed 4-bit weights (uint8 [..., ceil(N / 16), K / 128, tile]) with a bf16 scale per row
+    and ``group_size`` columns (32, 64 or 128): scale = bf16(max|w| / 7), q = clamp(rint(w / scale), -8, 7).
+
+    ``w``: bfloat16, float16 or float32, or float8_e4m3fn with the operator's 128x128 ``block_scale``
+    (fp32 [..., ceil(N / 128), K / 128]).  ``scale`` (bf16 [..., N, K / group_size], positive) gives the scales instead,
+    so that weights which already are q * scale are packed exactly.  A group holding a NaN or an infinity gets the
+    scale NaN; one whose scale is zero or below the smallest normal number gets zeros."""
+    _require(isinstance(w, torch.Tensor) and w.dtype in _W4_TYPES, "w must be bfloat16, float16, float32 or float8_e4m3fn")
+    _require(w.dim() >= 2 and w.is_contiguous(), "w must be contiguous [..., N, K]")
+    _require(group_size in (32, 64, 128), "group_size must be 32, 64 or 128")
+    N, K = w.size(-2), w.size(-1)
+    _require(N > 0 and K > 0 and K % 128 == 0, "K must be a positive multiple of 128 and N positive")
+    lead = tuple(w.shape[:-2])
+    _require((block_scale is not None) == (w.dtype == torch.float8_e4m3fn),
+             "block_scale goes with float8_e4m3fn weights, and only with them")
+    if block_scale is not None:
+        _require(block_scale.dtype == torch.float32 and block_scale.is_contiguous()
+                 and tuple(block_scale.shape) == lead + ((N + 127) // 128, K // 128) and block_scale.device == w.device,
+                 "block_scale must be contiguous float32 [..., ceil(N / 128), K / 128] on w's device")
+    if scale is not None:
+        _require(scale.dtype == torch.bfloat16 and scale.is_contiguous()
+                 and tuple(scale.shape) == lead + (N, K // group_size) and scale.device == w.device,
+                 "scale must be contiguous bfloat16 [..., N, K / group_size] on w's device")
+    _require(w.is_cuda, "w must be a CUDA tensor")
+    packed = torch.empty(lead + ((N + 15) // 16, K // 128, 1024 + 4096 // group_size), dtype=torch.uint8,
+                         device=w.device)
+    if packed.numel():
+        _launch_on(w.device, load_library().fbmoe_quantize_w4, w.data_ptr(), _W4_TYPES[w.dtype],
+                   block_scale.data_ptr() if block_scale is not None else None,
+                   scale.data_ptr() if scale is not None else None, w.numel() // (N * K), N, K, group_size,
+                   packed.data_ptr())
+    return packed
+
+
+def dequantize_w4(packed: torch.Tensor, n: int = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Packed 4-bit weights -> [..., n, K] in ``dtype`` (bfloat16, float16 or float32): q * scale, rounded once.  ``n``:
+    the matrix's rows where they are not a multiple of 16."""
+    n, K, group = _w4_shape(packed, "packed", n)
+    _require(dtype in _W4_TYPES and dtype != torch.float8_e4m3fn, "dtype must be bfloat16, float16 or float32")
+    _require(packed.is_cuda, "packed must be a CUDA tensor")
+    out = torch.empty(tuple(packed.shape[:-3]) + (n, K), dtype=dtype, device=packed.device)
+    if out.numel():
+        _launch_on(packed.device, load_library().fbmoe_dequantize_w4, packed.data_ptr(), out.numel() // (n * K), n, K,
+                   group, _W4_TYPES[dtype], out.data_ptr())
+    return out
+
+
+def linear_w4(x: torch.Tensor, weight: torch.Tensor, n: int = None, out: torch.Tensor = None) -> torch.Tensor:
+    """``x @ W^T`` for at most 64 tokens: x [T, K] bfloat16 or float16 (rows may be strided by a multiple of 8
+    elements), ``weight`` one packed [n, K] matrix; returns [T, n] in x's type, summed in fp32.  More tokens: a GEMM
+    on ``dequantize_w4(weight, n)``."""
+    n, K, group = _w4_shape(weight, "weight", n)
+    _require(weight.dim() == 3, "weight must be one packed matrix [ceil(N / 16), K / 128, tile]")
+    _require(isinstance(x, torch.Tensor) and x.dtype in (torch.bfloat16, torch.float16),
+             "x must be bfloat16 or float16")
+    _require(x.dim() == 2 and x.size(1) == K, f"x must be [T, {K}]")
+    T = x.size(0)
+    _require(T <= W4_MAX_TOKENS, f"linear_w4 takes at most {W4_MAX_TOKENS} tokens; use a GEMM on dequantize_w4(weight)")
+    x_stride = x.stride(0) if T > 1 else K
+    _require(x.stride(1) == 1 and x_stride >= K and x_stride % 8 == 0,
+             "x's rows must be contiguous and a multiple of 8 elements apart")
+    _require(x.is_cuda and weight.is_cuda and x.device == weight.device, "x and weight must be on one CUDA device")
+    if out is None:
+        out = torch.empty((T, n), dtype=x.dtype, device=x.device)
+    else:
+        _require(out.dtype == x.dtype and tuple(out.shape) == (T, n) and out.device == x.device
+                 and out.stride(1) == 1 and (T <= 1 or out.stride(0) >= n),
+                 "out must be [T, n] in x's type on x's device, its rows contiguous")
+    if T:
+        _launch_on(x.device, load_library().fbmoe_linear_w4, x.data_ptr(), x_stride, _W4_TYPES[x.dtype], T,
+                   weight.data_ptr(), n, K, group, out.data_ptr(), out.stride(0) if T > 1 else n)
+    return out
+
+
+def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2_weights, local_expert_offset,
+               routed_scaling_factor, out: torch.Tensor = None) -> torch.Tensor:
+    """The fused MoE layer for at most 64 tokens on packed 4-bit weights: ``hidden_states`` [T, H] bfloat16 or float16,
+    ``gemm1_weights`` E_local packed [2I, H] matrices (rows [0, I) the linear half, [I, 2I) the silu half),
+    ``gemm2_weights`` E_local packed [H, I] matrices, routing as ``forward``; returns [T, H] in hidden_states' type.
+    The workspace is allocated per call, so calls may overlap and captured graphs share nothing."""
+    N1, H, group1 = _w4_shape(gemm1_weights, "gemm1_weights")
+    N2, I, group2 = _w4_shape(gemm2_weights, "gemm2_weights")
+    x = hidden_states
+    _require(gemm1_weights.dim() == 4 and gemm2_weights.dim() == 4 and gemm1_weights.size(0) == gemm2_weights.size(0)
+             and 1 <= gemm1_weights.size(0) <= E_GLOBAL,
+             "gemm1_weights and gemm2_weights must hold the same 1..256 packed matrices")
+    _require(N1 == 2 * I and N2 == H, f"gemm1_weights must be packed [2I, H] and gemm2_weights packed [H, I]; they are "
+                                      f"[{N1}, {H}] and [{N2}, {I}]")
+    _require(isinstance(x, torch.Tensor) and x.dtype in (torch.bfloat16, torch.float16) and x.dim() == 2
+             and x.size(1) == H and x.is_contiguous(), f"hidden_states must be contiguous bfloat16 or float16 [T, {H}]")
+    T, E = x.size(0), gemm1_weights.size(0)
+    _require(T <= W4_MAX_TOKENS, f"fused_moe_w4 takes at most {W4_MAX_TOKENS} tokens")
+    _require(isinstance(routing_logits, torch.Tensor) and routing_logits.dtype == torch.float32
+             and tuple(routing_logits.shape) == (T, E_GLOBAL) and routing_logits.is_contiguous(),
+             "routing_logits must be contiguous float32 [T, 256]")
+    _require(isinstance(routing_bias, torch.Tensor) and routing_bias.dtype == torch.bfloat16
+             and routing_bias.numel() == E_GLOBAL and routing_bias.is_contiguous(),
+             "routing_bias must be 256 contiguous bfloat16")
+    offset = int(local_expert_offset)
+    _require(0 <= offset < E_GLOBAL, "local_expert_offset must be in 0..255")
+    dev = x.device
+    _require(all(t.is_cuda and t.device == dev for t in (routing_logits, routing_bias, x, gemm1_weights, gemm2_weights)),
+             "all tensors must be on one CUDA device")
+    if out is None:
+        out = torch.empty((T, H), dtype=x.dtype, device=dev)
+    else:
+        _require(out.dtype == x.dtype and tuple(out.shape) == (T, H) and out.is_contiguous() and out.device == dev,
+                 "out must be contiguous [T, H] in hidden_states' type on its device")
+    if T:
+        lib = load_library()
+        ws = torch.empty(lib.fbmoe_w4_workspace_size(T, H, I), dtype=torch.uint8, device=dev)
+        _launch_on(dev, lib.fbmoe_forward_w4, routing_logits.data_ptr(), routing_bias.data_ptr(), x.data_ptr(),
+                   _W4_TYPES[x.dtype], gemm1_weights.data_ptr(), group1, gemm2_weights.data_ptr(), group2, T, H, I, E,
+                   offset, float(routed_scaling_factor), out.data_ptr(), ws.data_ptr(), ws.numel())
+    return out
 
 
 # ---------------------------------------------------------------- expert parallelism over peer memory

@@ -55,3 +55,26 @@ def fused_moe(
         int(local_expert_offset),
         float(routed_scaling_factor),
     )
+
+
+@torch.no_grad()
+def fused_moe_w4(
+    routing_logits: torch.Tensor,
+    routing_bias: torch.Tensor,
+    hidden_states: torch.Tensor,
+    gemm1_weights: torch.Tensor,
+    gemm2_weights: torch.Tensor,
+    local_expert_offset: int,
+    routed_scaling_factor: float,
+):
+    """The same layer for at most 64 tokens on 4-bit weights packed by ``fbmoe_lib.quantize_w4``: ``hidden_states``
+    bfloat16 or float16 ``[T, H]``, any H and I that are multiples of 128; returns ``[T, H]`` in its type."""
+    return _fbmoe.forward_w4(
+        routing_logits,
+        routing_bias,
+        hidden_states,
+        gemm1_weights,
+        gemm2_weights,
+        local_expert_offset,
+        routed_scaling_factor,
+    )

@@ -296,6 +296,56 @@ FBMOE_API int fbmoe_ipc_handle(const void* ptr, void* handle_out);
 FBMOE_API int fbmoe_ipc_open(const void* handle, void** ptr);
 FBMOE_API int fbmoe_ipc_close(void* ptr);
 
+/* ---- 4-bit weights with group scales for a few tokens (no counterpart in the
+ * reference, whose weights are fp8).
+ *
+ * Packed format: a matrix [N, K] (K a multiple of 128) is cut into tiles of 16
+ * rows by 128 columns, stored [ceil(N / 16)][K / 128][tile]; a stack of `batch`
+ * matrices one after another.  A tile is 1024 bytes of 4-bit values u = q + 8 (q in
+ * [-8, 7]) and 4096 / group bytes of bf16 scales; the weight is q * scale.
+ * Values: 256 little-endian 32-bit words ordered [h 2][g 8][t 4][j 4]; word
+ * (h, g, t, j) holds row 8h + g, columns 32j + 8t .. + 7 as
+ * rotl32(sum over i < 4 of u[2i] << 4i | u[2i + 1] << (16 + 4i), 3).  Scales:
+ * [128 / group][g 8][h 2].  Rows past N hold zeros.  group: 32, 64 or 128 columns. */
+enum { FBMOE_BF16 = 0, FBMOE_F16 = 1, FBMOE_F32 = 2, FBMOE_E4M3 = 3 }; /* element types */
+
+/* Bytes of `batch` packed matrices (0 for sizes the format does not take). */
+FBMOE_API size_t fbmoe_w4_bytes(int64_t batch, int N, int K, int group);
+
+/* w [batch, N, K] of type w_type -> packed.  Per row and group: scale =
+ * bf16(max |w| / 7), 0 when that is below the smallest normal number;
+ * q = clamp(rint(w / scale), -8, 7) with the IEEE fp32 quotient.  scale_bf16
+ * [batch, N, K / group] gives the scales instead (weights that already are
+ * q * scale come back exactly); where it is not a positive normal number q is 0.
+ * A group that holds a NaN or an infinity gets the scale NaN.  FBMOE_E4M3 weights
+ * are multiplied by block_scale [batch, ceil(N / 128), K / 128] (the operator's own
+ * 128x128 scales).  w and packed 16-byte aligned. */
+FBMOE_API int fbmoe_quantize_w4(const void* w, int w_type, const float* block_scale, const void* scale_bf16,
+                                int64_t batch, int N, int K, int group, void* packed, void* stream);
+
+/* packed -> out [batch, N, K] of out_type (not FBMOE_E4M3): q * scale, rounded once. */
+FBMOE_API int fbmoe_dequantize_w4(const void* packed, int64_t batch, int N, int K, int group, int out_type, void* out,
+                                  void* stream);
+
+/* out[t, n] = sum over k of x[t, k] * w[n, k] for 0 <= T <= 64 tokens: x and out of
+ * `type` (FBMOE_BF16 or FBMOE_F16), rows x_stride and out_stride elements apart
+ * (x 16-byte aligned, x_stride a multiple of 8), sums in fp32. */
+FBMOE_API int fbmoe_linear_w4(const void* x, int64_t x_stride, int type, int T, const void* packed, int N, int K,
+                              int group, void* out, int64_t out_stride, void* stream);
+
+/* The fused MoE layer on packed 4-bit weights for 0 <= T <= 64 tokens: routing as
+ * fbmoe_forward (256 experts, top-8), hidden_states and out [T, H] of `type`
+ * (FBMOE_BF16 or FBMOE_F16), gemm1_weights E_local packed [2I, H] matrices (rows
+ * [0, I) the linear half, [I, 2I) the silu half), gemm2_weights E_local packed
+ * [H, I] matrices; H and I multiples of 128; sums in fp32, the result rounded
+ * once.  Pointers 16-byte aligned; workspace >= fbmoe_w4_workspace_size(T, H, I)
+ * bytes, 256-byte aligned; calls that may overlap need a workspace each. */
+FBMOE_API size_t fbmoe_w4_workspace_size(int T, int H, int I);
+FBMOE_API int fbmoe_forward_w4(const float* routing_logits, const void* routing_bias, const void* hidden_states,
+                               int type, const void* gemm1_weights, int group1, const void* gemm2_weights, int group2,
+                               int T, int H, int I, int E_local, int local_expert_offset, float routed_scaling_factor,
+                               void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 FBMOE_API const char* fbmoe_error_string(int code);
 
 /* Library version (major*10000 + minor*100 + patch). */
