@@ -52,11 +52,25 @@ struct F16 {
   static __device__ __forceinline__ Raw of(float v) { return __float2half_rn(v); }
 };
 
+// (v & mask) | magic in one instruction: an instruction holds one 32-bit constant, so the other one has to be in a
+// register, where the compiler does not put it by itself (it makes two instructions of the expression).
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x00780078, %2, 0xEA;" : "=r"(r) : "r"(v), "r"(magic));
+  return r;
+}
+template <typename A>
+__device__ __forceinline__ uint32_t magic_register() {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "n"(A::kMagic));
+  return r;
+}
+
 // The word's four pairs (q[2i], q[2i + 1]) as exact 16-bit floats.
 template <typename A>
-__device__ __forceinline__ void decode_word(uint32_t w, uint32_t (&p)[4]) {
+__device__ __forceinline__ void decode_word(uint32_t w, uint32_t magic, uint32_t (&p)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = A::minus_bias((__funnelshift_r(w, w, 4 * i) & 0x00780078u) | A::kMagic);
+  for (int i = 0; i < 4; ++i) p[i] = A::minus_bias(and_or(i ? __funnelshift_r(w, w, 4 * i) : w, magic));
 }
 
 // c (16 x 8, fp32) += a (16 x 16) * b (16 x 8).
@@ -86,7 +100,7 @@ __device__ __forceinline__ void mma_16816<F16>(float (&c)[4], uint32_t a0, uint3
 // sum is multiplied by its fp32 scale.  acc[n][0..1] are row g, columns 8n + 2t, + 1; acc[n][2..3] row g + 8.
 template <typename A, int G, int NT>
 __device__ __forceinline__ void tile_product(const uint4& qlo, const uint4& qhi, const uint32_t (&scales)[128 / G],
-                                             const uint4 (&x)[NT][4], float (&acc)[NT][4]) {
+                                             const uint4 (&x)[NT][4], uint32_t magic, float (&acc)[NT][4]) {
   const uint32_t wl[4] = {qlo.x, qlo.y, qlo.z, qlo.w}, wh[4] = {qhi.x, qhi.y, qhi.z, qhi.w};
 #pragma unroll
   for (int gr = 0; gr < 128 / G; ++gr) {
@@ -98,8 +112,8 @@ __device__ __forceinline__ void tile_product(const uint4& qlo, const uint4& qhi,
 #pragma unroll
     for (int j = gr * (G / 32); j < (gr + 1) * (G / 32); ++j) {
       uint32_t pl[4], ph[4];
-      decode_word<A>(wl[j], pl);
-      decode_word<A>(wh[j], ph);
+      decode_word<A>(wl[j], magic, pl);
+      decode_word<A>(wh[j], magic, ph);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         mma_16816<A>(c[n], pl[0], ph[0], pl[1], ph[1], x[n][j].x, x[n][j].y);

@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(kWarps * 32) linear_kernel(const typename A::R
         xv[n][j] = row < T ? __ldg(reinterpret_cast<const uint4*>(x + (size_t)row * ldx + kt * kTileK + 32 * j + 8 * t))
                            : make_uint4(0, 0, 0, 0);
     }
-    tile_product<A, G, NT>(qlo, qhi, sw, xv, acc);
+    tile_product<A, G, NT>(qlo, qhi, sw, xv, magic_register<A>(), acc);
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n)

@@ -192,6 +192,7 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* 
     const uint8_t* in = packed + (size_t)tile * tile_bytes(G);
     const uint4 q[2] = {__ldg(reinterpret_cast<const uint4*>(in + 16 * lane)),
                         __ldg(reinterpret_cast<const uint4*>(in + 512 + 16 * lane))};
+    const uint32_t magic = magic_register<Bf16>();
     uint32_t sw[128 / G];
 #pragma unroll
     for (int gr = 0; gr < 128 / G; ++gr) sw[gr] = __ldg(reinterpret_cast<const uint32_t*>(in + kTileQ + 32 * gr + 4 * g));
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* 
         const uint32_t s2 = sw[j * 32 / G];
         const float s = h == 0 ? __uint_as_float(s2 << 16) : __uint_as_float(s2 & 0xFFFF0000u);
         uint32_t p[4];
-        decode_word<Bf16>(w[j], p);
+        decode_word<Bf16>(w[j], magic, p);
         float v[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -120,7 +120,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.fbmoe_w4_workspace_size.argtypes = [i32, i32, i32]
         lib.fbmoe_w4_workspace_size.restype = sz
         lib.fbmoe_forward_w4.argtypes = [vp, vp, vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, vp, vp, sz,
-                                         vp]
+                                         vp, vp]
         lib.fbmoe_forward_w4.restype = i32
         lib.fbmoe_ipc_alloc.argtypes = [sz, ctypes.POINTER(vp)]
         lib.fbmoe_ipc_alloc.restype = i32
@@ -554,12 +554,31 @@ def linear_w4(x: torch.Tensor, weight: torch.Tensor, n: int = None, out: torch.T
     return out
 
 
+def _w4_sink(dev: torch.device):
+    """(key, address) of the device's status sink for forward_w4: one pinned word that lives as long as the process.  A
+    capture cannot allocate it; a graph captured before the device's first call reports no status."""
+    key = (dev.index, -1)
+    sink = _sinks.get(key)
+    if sink is None:
+        if torch.cuda.is_current_stream_capturing():
+            return key, None
+        with _ws_lock:
+            if key not in _sinks:
+                sink = torch.zeros(1, dtype=torch.int32).pin_memory()
+                _sink_words[key] = ctypes.c_uint32.from_address(sink.data_ptr())
+                _sinks[key] = sink
+            sink = _sinks[key]
+    return key, sink.data_ptr()
+
+
 def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2_weights, local_expert_offset,
-               routed_scaling_factor, out: torch.Tensor = None) -> torch.Tensor:
+               routed_scaling_factor, out: torch.Tensor = None, sync_status: bool = None) -> torch.Tensor:
     """The fused MoE layer for at most 64 tokens on packed 4-bit weights: ``hidden_states`` [T, H] bfloat16 or float16,
     ``gemm1_weights`` E_local packed [2I, H] matrices (rows [0, I) the linear half, [I, 2I) the silu half),
     ``gemm2_weights`` E_local packed [H, I] matrices, routing as ``forward``; returns [T, H] in hidden_states' type.
-    The workspace is allocated per call, so calls may overlap and captured graphs share nothing."""
+    The workspace is allocated per call, so calls may overlap and captured graphs share nothing.  Device-side errors
+    (a bounded wait that expired) raise DeviceStatusError as in ``forward``: at a later call on the device or at
+    check_status(), or for this call with ``sync_status`` (or FBMOE_SYNC_STATUS=1)."""
     N1, H, group1 = _w4_shape(gemm1_weights, "gemm1_weights")
     N2, I, group2 = _w4_shape(gemm2_weights, "gemm2_weights")
     x = hidden_states
@@ -590,10 +609,19 @@ def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2
                  "out must be contiguous [T, H] in hidden_states' type on its device")
     if T:
         lib = load_library()
+        key, sink = _w4_sink(dev)
+        word = _take_sink(key)
+        if word:
+            raise DeviceStatusError(word, "reported by an earlier forward_w4 on this device")
         ws = torch.empty(lib.fbmoe_w4_workspace_size(T, H, I), dtype=torch.uint8, device=dev)
         _launch_on(dev, lib.fbmoe_forward_w4, routing_logits.data_ptr(), routing_bias.data_ptr(), x.data_ptr(),
                    _W4_TYPES[x.dtype], gemm1_weights.data_ptr(), group1, gemm2_weights.data_ptr(), group2, T, H, I, E,
-                   offset, float(routed_scaling_factor), out.data_ptr(), ws.data_ptr(), ws.numel())
+                   offset, float(routed_scaling_factor), out.data_ptr(), ws.data_ptr(), ws.numel(), sink)
+        if sync_status_default() if sync_status is None else sync_status:
+            torch.cuda.current_stream(dev).synchronize()
+            word = _take_sink(key)
+            if word:
+                raise DeviceStatusError(word, "reported by this forward_w4")
     return out
 
 

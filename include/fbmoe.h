@@ -339,12 +339,16 @@ FBMOE_API int fbmoe_linear_w4(const void* x, int64_t x_stride, int type, int T, 
  * [0, I) the linear half, [I, 2I) the silu half), gemm2_weights E_local packed
  * [H, I] matrices; H and I multiples of 128; sums in fp32, the result rounded
  * once.  Pointers 16-byte aligned; workspace >= fbmoe_w4_workspace_size(T, H, I)
- * bytes, 256-byte aligned; calls that may overlap need a workspace each. */
+ * bytes, 256-byte aligned; calls that may overlap need a workspace each.  A bounded
+ * wait that expires sets the status word at the workspace's start (the bits of
+ * fbmoe_read_status) and stores it to status_sink (device-accessible, e.g. pinned host memory;
+ * sticky; may be NULL). */
 FBMOE_API size_t fbmoe_w4_workspace_size(int T, int H, int I);
 FBMOE_API int fbmoe_forward_w4(const float* routing_logits, const void* routing_bias, const void* hidden_states,
                                int type, const void* gemm1_weights, int group1, const void* gemm2_weights, int group2,
                                int T, int H, int I, int E_local, int local_expert_offset, float routed_scaling_factor,
-                               void* out, void* workspace, size_t workspace_bytes, void* stream);
+                               void* out, void* workspace, size_t workspace_bytes, uint32_t* status_sink,
+                               void* stream);
 
 FBMOE_API const char* fbmoe_error_string(int code);
 

@@ -28,6 +28,15 @@ def half_step(y, dtype):
     return y.abs() * (info.eps / 2) + info.smallest_normal * info.eps  # subnormal results: their absolute step
 
 
+def plane_error(x, block):
+    """What is lost of x [.., K] as 16-bit integers: per `block` columns in units of s, the power of two that puts the
+    largest magnitude m, times 1 + 2^-7, into [2^14, 2^15)."""
+    b = x.double().view(*x.shape[:-1], -1, block)
+    m = b.abs().amax(-1, keepdim=True) * (1 + 2.0 ** -7)
+    s = torch.where(m > 0, 2.0 ** (torch.floor(torch.log2(m)) - 14), torch.ones_like(m))
+    return (b - torch.round(b / s) * s).abs().view(x.shape)
+
+
 def random_packed(N, K, G, seed, lead=(), q_range=(-8, 8)):
     """Packed random weights of about unit row norm, and their 64-bit values [lead.., N, K] on the GPU."""
     g = torch.Generator().manual_seed(seed)
@@ -225,11 +234,14 @@ class Case:
         return (self.logits, self.bias, self.x, self.w1, self.w2, self.offset, 2.5)
 
     def check(self, y):
-        """The layer in 64 bits and its error bound.  d1 bounds the error of both halves of the first product; through
-        h = silu(g) u (|silu'| < 1.1, |silu(g)| <= |g|) it reaches h, which is also rounded by expf, a division and two
-        products (2^-20 in all) and kept to 2^-16; the second product's own sums follow; each output is a sum of up to
-        8 weighted pairs (16 * 2^-24), rounded once.  The weights come from lib.route in fp32 as the kernel's do."""
+        """The layer in 64 bits and its error bound.  d1 bounds the error of both halves of the first product: its sums,
+        and x as 16-bit integers.  Through h = silu(g) u (|silu'| < 1.1, |silu(g)| <= |g|) it reaches h, which is also
+        rounded by expf, a division and two products (2^-20 in all) and kept as a 16-bit integer: half a unit, and the
+        unit is at most 2^-14 (1 + 2^-6) of the largest of 32.  The second product's own sums follow; each output is a
+        sum of up to 8 weighted pairs (16 * 2^-24), rounded once.  The weights come from lib.route in fp32 as the
+        kernel's do."""
         assert y.dtype == self.x.dtype and tuple(y.shape) == (self.T, self.H)
+        lost = plane_error(self.x, 128)
         for t in range(self.T):
             ref = torch.zeros(self.H, dtype=torch.float64, device="cuda")
             err = torch.zeros_like(ref)
@@ -238,11 +250,13 @@ class Case:
                     continue
                 v1, v2, x = self.v1[e - self.offset], self.v2[e - self.offset], self.x[t].double()
                 a, size = v1 @ x, v1.abs() @ x.abs()
-                d1 = steps(self.H, self.G1) * size
+                d1 = steps(self.H, self.G1) * size + v1.abs() @ lost[t]
                 u, gate = a[:self.I], a[self.I:]
                 silu = gate / (1 + torch.exp(-gate))
                 h = silu * u
-                dh = 1.1 * d1[self.I:] * (u.abs() + d1[:self.I]) + silu.abs() * d1[:self.I] + (2.0 ** -16 + 2.0 ** -20) * h.abs()
+                dh = 1.1 * d1[self.I:] * (u.abs() + d1[:self.I]) + silu.abs() * d1[:self.I] + 2.0 ** -20 * h.abs()
+                top = (h.abs() + dh).view(-1, 32).amax(-1).repeat_interleave(32)
+                dh = dh + top * (2.0 ** -15 * (1 + 2.0 ** -6))
                 ref += w * (v2 @ h)
                 err += abs(w) * (v2.abs() @ dh + (2 * steps(self.I, self.G2) + 2.0 ** -20) * (v2.abs() @ h.abs()))
             tol = half_step(ref, y.dtype) * (1 + 2.0 ** -8) + err
@@ -387,9 +401,28 @@ def test_workspace_contents_do_not_matter(fbmoe_lib, fill):
     out = torch.empty_like(want)
     for _ in range(2):
         rc = lib.fbmoe_forward_w4(c.logits.data_ptr(), c.bias.data_ptr(), c.x.data_ptr(), 0, c.w1.data_ptr(), 128,
-                                  c.w2.data_ptr(), 64, 7, 512, 256, 32, 64, 2.5, out.data_ptr(), ws.data_ptr(), n,
+                                  c.w2.data_ptr(), 64, 7, 512, 256, 32, 64, 2.5, out.data_ptr(), ws.data_ptr(), n, None,
                                   torch.cuda.current_stream().cuda_stream)
         assert rc == 0
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     assert (ws[n:] == fill).all()
+
+
+def test_expired_wait_is_reported(fbmoe_lib):
+    """A down unit that waits for one arrival that never comes gives up, and the call says so."""
+    lib = fbmoe_lib.load_library()
+    c = Case(fbmoe_lib, 4, 32, 0, 256, 128, 64, 64, BF16, "group", 77)
+    want = fbmoe_lib.forward_w4(*c.args(), sync_status=True)
+    lib.fbmoe_test_expire_grid_wait(1)
+    try:
+        with pytest.raises(fbmoe_lib.DeviceStatusError) as e:
+            fbmoe_lib.forward_w4(*c.args(), sync_status=True)
+        assert e.value.word & 4
+        fbmoe_lib.forward_w4(*c.args())
+        with pytest.raises(fbmoe_lib.DeviceStatusError):
+            fbmoe_lib.check_status()
+    finally:
+        lib.fbmoe_test_expire_grid_wait(0)
+    torch.cuda.synchronize()
+    assert torch.equal(fbmoe_lib.forward_w4(*c.args(), sync_status=True), want)

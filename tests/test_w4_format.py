@@ -123,11 +123,11 @@ def test_c_entry_points_refuse(fbmoe_lib):
     assert size(65, 128, 128) == 0 and size(-1, 128, 128) == 0 and size(1, 100, 128) == 0 and size(1, 128, 0) == 0
     assert 0 < size(1, 128, 128) < size(64, 7168, 2048)
 
-    def m(T=1, H=128, I=128, E=1, off=0, type_=0, g1=64, g2=64, p=a16, ws=4096, n=1 << 30):
-        return lib.fbmoe_forward_w4(p, p, p, type_, p, g1, p, g2, T, H, I, E, off, 2.5, p, ws, n, nul)
+    def m(T=1, H=128, I=128, E=1, off=0, type_=0, g1=64, g2=64, p=a16, ws=4096, n=1 << 30, sink=nul):
+        return lib.fbmoe_forward_w4(p, p, p, type_, p, g1, p, g2, T, H, I, E, off, 2.5, p, ws, n, sink, nul)
 
     assert m(T=0) == 0 and m(p=nul) == -3 and m(ws=nul) == -3 and m(p=a16 + 4) == -4 and m(ws=4096 + 16) == -4
-    assert m(n=1) == -2
+    assert m(n=1) == -2 and m(sink=4097) == -4
     for bad in (dict(T=65), dict(T=-1), dict(H=64), dict(I=200), dict(E=0), dict(E=257), dict(off=-1), dict(off=256),
                 dict(type_=2), dict(g1=16), dict(g2=256), dict(H=1 << 21)):
         assert m(**bad) == -1, bad
