@@ -65,6 +65,11 @@ inline cudaError_t set_max_dynamic_smem(Kernel kernel, int bytes, DeviceFlags& d
   return e;
 }
 
+int num_sms_of_current_device();
+// 4-D map of 8-byte elements without swizzle; strides in bytes.  FBMOE_OK or FBMOE_ERR_DRIVER.
+int encode_4d_words(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
+                    const uint32_t (&box)[4]);
+
 // Offsets (bytes) of the sub-buffers inside the caller-provided workspace.
 struct Layout {
   size_t status;       // uint32[4]  device status word(s)

@@ -8,16 +8,19 @@
 //
 // route_kernel: one CTA per token; a warp routes it, all make its planes; also zeroes the layer kernel's counters.
 //
-// layer_kernel: one CTA of 16 warps per SM.  Groups of P warps, P chosen so that there are about as many groups as
-// tasks, work alone on tasks handed out by a ticket counter in the order
-//   up: (up to 8 rows of an expert; 32 pairs of W1 rows, two linear and two silu tiles side by side),
-//   down: (up to 8 rows of an expert; 32 rows of W2),
-//   combine: 128 P outputs.
-// A group's warps split K and join their partial sums in shared memory.  Each warp streams its part's tiles through its
-// ring, and a group knows its tickets ahead of what it works on, so the stream does not stop between tasks or phases.  A
-// down task needs its expert's up tasks, a combine task all down tasks.  Tickets are taken in order, so whatever a task
-// waits for has been taken by a group that is running already and that waits for less: no co-residency is assumed, and
-// two calls may share the GPU.  Every order of summation depends on the sizes and the numbers of row blocks alone.
+// layer_kernel: one CTA per SM, working on units handed out by a ticket counter in the order
+//   up: (up to 8 rows of an expert; 32 MW pairs of W1 rows, two linear and two silu tiles side by side),
+//   down: (up to 8 rows of an expert; 64 MW rows of W2),
+//   combine: 2048 outputs.
+// A down unit needs its expert's up units, a combine unit all down units.  Tickets are taken in order, so whatever a unit
+// waits for has been taken by a CTA that is running already and that waits for less: no co-residency is assumed, and two
+// calls may share the GPU.
+//
+// The scheduler warp takes tickets ahead and waits for what a unit needs; 16 consumer warps, KW along K times MW along
+// the rows, stream the unit's tiles through their rings (w4_stream.cuh) and on into the next unit's; two finisher warps
+// add their partial sums in a fixed order, apply SwiGLU or the routing weight, store and report.  A unit takes an SM 3 to
+// 6 us at H = 7168, so phases and the end of the call are balanced to that; with a unit per warp or group of warps
+// (measured) they were not: 207 us in place of TODO64 us at T = 64.  Every order of summation depends on the sizes alone.
 #include "fbmoe.h"
 #include "fbmoe_launch.h"
 #include "moe_route.cuh"
@@ -27,17 +30,21 @@ namespace fbmoe {
 namespace w4 {
 namespace {
 
-constexpr int kRows = 8;                    // token rows of a task
-constexpr int kSpan = 2 * kTileN;           // rows of h that an up task makes, and of W2 that a down task takes
-constexpr int kThreads = kStreamWarps * 32;
-constexpr int kCombine = 128;               // outputs of a combine task
+constexpr int kRows = 8;                    // token rows of a unit
+constexpr int kUpSpan = 32, kDownSpan = 64;   // columns of h, rows of W2 of a consumer warp (four tiles)
+constexpr int kFinishers = 2;
+constexpr int kThreads = (kStreamWarps + 4) * 32;  // consumers; finishers, scheduler, one idle
+// Registers: five warps per quarter of an SM are launched with 96 each; the fifth gives up 32, the consumers take 8.
+constexpr int kConsumerRegs = 104, kHelperRegs = 64;
+constexpr int kCombine = 4 * 32 * kStreamWarps;  // outputs of a combine unit
+constexpr int kQueue = 2;                   // units known: the one worked on, and the one whose tiles are under way
 constexpr int kMaxBlocks = kMaxTokens * kTopK / kRows + kExperts;  // row blocks of all experts
-constexpr int kPart = 256;                  // floats of a warp's partial sums that are joined at a time
+constexpr int kPart = 512;                  // floats of a consumer warp's partial sums: [4 tokens][half][lane][4]
 
 // counters in the workspace, zeroed by route_kernel
 struct Counters {
   uint32_t status, ticket, done, pad;
-  uint32_t ready[kExperts];  // finished up tasks of each local expert
+  uint32_t ready[kExperts];  // finished (up unit, finisher) pairs of each local expert
 };
 
 struct MoeLayout {
@@ -134,8 +141,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const float* __res
 }
 
 struct LayerArgs {
-  const uint8_t *w1, *w2;
+  CUtensorMap map1, map2;  // W1, W2
   int T, H, I, E, offset;
+  int kw1[2], kw2[2];    // consumer warps along K of an up / down unit: for small calls, for large ones
   int depth;             // steps of a ring
   const int32_t* topk_idx;
   const float* topk_w;
@@ -146,7 +154,7 @@ struct LayerArgs {
   Counters* counters;
   void* out;
   uint32_t* sink;
-  uint64_t wait_ns;      // limit of a wait for other warps' tasks
+  uint64_t wait_ns;      // limit of a wait for other CTAs' units
   uint32_t extra;        // arrivals that never come (test hook)
 };
 
@@ -154,27 +162,29 @@ struct LayerArgs {
 __device__ __forceinline__ uint32_t block_word(int e, int pos, int rows) { return e | pos << 8 | rows << 20; }
 __device__ __forceinline__ int block_expert(uint32_t w) { return w & 0xff; }
 __device__ __forceinline__ int block_pos(uint32_t w) { return w >> 8 & 0xfff; }
-__device__ __forceinline__ int block_rows_of(uint32_t w) { return w >> 20; }
+__device__ __forceinline__ int block_rows_of(uint32_t w) { return w >> 20 & 0xff; }
 
-// The tasks of a call.
-struct Plan {
-  int log_p;               // log2 of the warps of a group
-  uint32_t up_rows, n_up;  // row positions per row block, tasks
-  uint32_t down_rows, n_down;
-  uint32_t n_all;
+enum Kind { kStop = 0, kUp = 1, kDown = 2, kSum = 3 };
+// A unit: its row block, its place along the rows (or, to be summed, along the outputs).
+struct __align__(8) Unit {
+  uint32_t block;  // and the kind in bits 28, 29
+  uint32_t row;
 };
+__device__ __forceinline__ int kind_of(const Unit& u) { return u.block >> 28; }
 
 struct Shared {
   unsigned long long mask[kExperts];  // tokens of each local expert
   uint64_t ring_full[kStreamWarps][kMaxDepth];
-  uint32_t tickets[kStreamWarps][4];   // a group's tasks: the one it works on, the next, and the one after that
-  float part[kStreamWarps][kPart];
+  uint64_t known[kQueue], go[kQueue], done[kQueue];  // a queue slot's unit is there; may be begun; is finished
+  uint64_t part_full[2], part_empty[2];
+  Unit unit[kQueue];
   uint32_t block[kMaxBlocks];
   uint32_t warp_sum[8];
   uint16_t pair_at[kExperts];          // first place of an expert's pairs
   uint16_t pairs[kMaxTokens * kTopK];  // token * 8 + slot, by expert, tokens ascending
+  float pair_w[kMaxTokens * kTopK];    // their weights
   int n_blocks;                        // row blocks
-  Plan plan;
+  int kw1, kw2;                        // the call's choice
   int abort;
 };
 
@@ -221,122 +231,84 @@ __device__ __forceinline__ void build_lists(const LayerArgs& a, Shared& s) {
     for (int r = 0; r < rows; r += kRows) s.block[block + r / kRows] = block_word(tid, pos + r, min(kRows, rows - r));
   }
   __syncthreads();
-  if (e >= 0) s.pairs[s.pair_at[e] + __popcll(s.mask[e] & ((1ull << (tid / kTopK)) - 1))] = (uint16_t)tid;
+  if (e >= 0) {
+    const int at = s.pair_at[e] + __popcll(s.mask[e] & ((1ull << (tid / kTopK)) - 1));
+    s.pairs[at] = (uint16_t)tid;
+    s.pair_w[at] = a.topk_w[tid];
+  }
   __syncthreads();
-}
-
-// P doubles while that leaves no more groups than tasks of the smaller phase, and every warp a K position.
-__device__ __forceinline__ Plan make_plan(const LayerArgs& a, const Shared& s) {
-  Plan p;
-  p.up_rows = a.I / kSpan;
-  p.n_up = s.n_blocks * p.up_rows;
-  p.down_rows = a.H / kSpan;
-  p.n_down = s.n_blocks * p.down_rows;
-  const uint32_t tasks = min(p.n_up, p.n_down), warps = gridDim.x * kStreamWarps;
-  const int k_tiles = min(a.H, a.I) / kTileK;
-  p.log_p = 0;
-  while (p.log_p < 4 && tasks << (p.log_p + 1) <= warps && k_tiles >> (p.log_p + 1) > 0) ++p.log_p;
-  p.n_all = p.n_up + p.n_down + (uint32_t)(((long)a.T * a.H + (kCombine << p.log_p) - 1) / (kCombine << p.log_p));
-  return p;
-}
-
-// A warp's part of a task.
-struct Task {
-  uint32_t block;    // row block
-  int row, k0, tiles;
-  const uint8_t* tile;
-};
-template <int G1, int G2>
-__device__ __noinline__ Task decode_task(const LayerArgs& a, const Shared& s, uint32_t ticket) {
-  const Plan& p = s.plan;
-  Task t;
-  const bool up = ticket < p.n_up;
-  const uint32_t rows = up ? p.up_rows : p.down_rows, at = up ? ticket : ticket - p.n_up, b = at / rows;
-  t.row = at - b * rows;
-  t.block = s.block[b];
-  const int kt = (up ? a.H : a.I) / kTileK, part = threadIdx.x / 32 & ((1 << p.log_p) - 1);
-  t.k0 = kt * part >> p.log_p;
-  t.tiles = (kt * (part + 1) >> p.log_p) - t.k0;
-  const size_t e = block_expert(t.block);
-  const size_t first = e * ((up ? 2 * a.I : a.H) / kTileN) + 2 * t.row;  // row tile
-  t.tile = (up ? a.w1 : a.w2) + (first * kt + t.k0) * (up ? tile_bytes(G1) : tile_bytes(G2));
-  return t;
-}
-
-// A warp's stream: the copies of its tasks' tiles, ahead of what it works on.  An up step is one K position of four row
-// tiles, a down step two K positions of two; lane i < copies holds the place of copy i.
-template <int G1, int G2>
-struct Stream {
-  Ring ring;
-  const uint8_t* src;
-  int left;              // steps of the task being issued that are still to be issued
-  int copies;
-  uint32_t bytes, last;  // of a copy, and of the task's last step
-  uint32_t task, known;  // tasks begun, and tasks whose tickets are known
-
-  // Issue the next steps while the ring has room.
-  __device__ __forceinline__ void fill(const LayerArgs& a, Shared& s) {
-    if (left > 1 && ring.free == 1) {  // the usual case: the step just released
-      ring.issue(src, copies, bytes, bytes);
-      src += bytes;
-      --left;
-      return;
-    }
-    fill_slow(a, s);
-  }
-  __device__ __forceinline__ void fill_slow(const LayerArgs& a, Shared& s) {
-    while (ring.free > 0) {
-      if (left == 0) {
-        if (task == known) return;
-        const uint32_t t = s.tickets[threadIdx.x / 32 >> s.plan.log_p][task % 4];
-        if (t >= s.plan.n_up + s.plan.n_down) return;  // no tiles from here on
-        ++task;
-        const Task k = decode_task<G1, G2>(a, s, t);
-        const int lane = threadIdx.x & 31;
-        if (t < s.plan.n_up) {
-          const size_t row = (size_t)(a.H / kTileK) * tile_bytes(G1);  // bytes of a row tile
-          src = k.tile + (lane & 1) * row + (lane >> 1 & 1) * (a.I / kTileN) * row;
-          copies = 4;
-          left = k.tiles;
-          bytes = last = tile_bytes(G1);
-        } else {
-          src = k.tile + (lane & 1) * (size_t)(a.I / kTileK) * tile_bytes(G2);
-          copies = 2;
-          left = (k.tiles + 1) / 2;
-          bytes = 2 * tile_bytes(G2);
-          last = k.tiles & 1 ? tile_bytes(G2) : bytes;
-        }
-      }
-      ring.issue(src, copies, left == 1 ? last : bytes, bytes);
-      src += bytes;
-      --left;
-    }
-  }
-};
-
-__device__ __forceinline__ void group_sync(int log_p) {
-  if (log_p == 0)
-    __syncwarp();
-  else
-    named_barrier_sync(1 + (threadIdx.x / 32 >> log_p), 32 << log_p);
 }
 
 __device__ __forceinline__ float swiglu(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
 
-// The sums of a group's partial values, in order, for its first warp (true).
-__device__ __forceinline__ bool join(Shared& s, int log_p, float (&v)[8]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-  if (log_p == 0) return true;
-  group_sync(log_p);  // the first warp has read what the last call left
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s.part[warp][32 * i + lane] = v[i];
-  group_sync(log_p);
-  if (warp & ((1 << log_p) - 1)) return false;
-  for (int w = 1; w < 1 << log_p; ++w)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += s.part[warp + w][32 * i + lane];
-  return true;
+// What a consumer warp has of a unit: K positions [k0, k0 + steps) of four row tiles.
+struct Span {
+  int k0, steps;
+};
+__device__ __forceinline__ Span span_of(const LayerArgs& a, const Shared& s, bool up) {
+  Span w;
+  const int kw = up ? s.kw1 : s.kw2, kt = (up ? a.H : a.I) / kTileK, kg = threadIdx.x / 32 & (kw - 1);
+  w.k0 = kt * kg / kw;
+  w.steps = kt * (kg + 1) / kw - w.k0;
+  return w;
 }
+// The warp's row group (32 columns of h, or 64 rows of W2) of a unit; it may lie past the last one.
+__device__ __forceinline__ uint32_t row_group(const Shared& s, const Unit& u, int warp) {
+  const int kw = kind_of(u) == kUp ? s.kw1 : s.kw2;
+  return u.row * (kStreamWarps / kw) + warp / kw;
+}
+__device__ __forceinline__ uint32_t row_groups(const LayerArgs& a, const Unit& u) {
+  return kind_of(u) == kUp ? a.I / kUpSpan : a.H / kDownSpan;
+}
+
+// A consumer warp's stream: the copies of its tiles, ahead of what it works on.  A step is one K position of four row
+// tiles, one tensor copy: a tile's bytes are kTileWords 8-byte elements, W1 maps as [expert][half][row tile][K position x
+// element] with boxes of two row tiles of both halves, W2 the same with one half and boxes of four.
+constexpr int tile_words(int group) { return tile_bytes(group) / 8; }
+template <int G1, int G2>
+struct Stream {
+  Ring ring;
+  const CUtensorMap* map;
+  int x, row, matrix;
+  int left;        // steps of the unit being issued that are still to be issued
+  uint32_t words;  // 8-byte elements of a tile
+  uint32_t seq;    // units begun
+  bool more;
+
+  __device__ __forceinline__ void step() {
+    ring.issue(map, x, row, 0, matrix, words * 32);
+    x += words;
+    --left;
+  }
+  // Issue steps while the ring has room.
+  __device__ __forceinline__ void fill(const LayerArgs& a, Shared& s) {
+    if (left > 0 && ring.free == 1) {  // the usual case: the step just released
+      step();
+      return;
+    }
+    while (ring.free > 0) {
+      if (left == 0) {
+        // the next unit, if it is known
+        if (!more || !__all_sync(0xffffffffu, Ring::test(smem_u32(&s.known[seq % kQueue]), seq / kQueue & 1))) return;
+        const Unit u = s.unit[seq % kQueue];
+        ++seq;
+        const int kind = kind_of(u);
+        more = kind == kUp || kind == kDown;
+        const uint32_t group = row_group(s, u, threadIdx.x / 32);
+        if (!more || group >= row_groups(a, u)) continue;
+        const Span w = span_of(a, s, kind == kUp);
+        words = kind == kUp ? tile_words(G1) : tile_words(G2);
+        map = kind == kUp ? &a.map1 : &a.map2;
+        x = w.k0 * words;
+        row = kind == kUp ? 2 * group : 4 * group;
+        matrix = block_expert(u.block);
+        left = w.steps;
+        continue;
+      }
+      step();
+    }
+  }
+};
 
 // The lane's places in the planes and scales of up to 4 NT tokens of a task (rows that are not there read the first
 // one's: their sums are not used), from K position k0 on.
@@ -361,16 +333,19 @@ struct Places {
       s[n] = scales + ((size_t)ps * kt_n + k0) * (FINE ? 4 : 1);
     }
   }
-  // The columns of the current K position.  x is constant while the kernel runs, h is not.
-  __device__ __forceinline__ void load(Columns<NT, FINE>& c) const {
+  // The current K position's words 2j, 2j + 1, and its scales.  x is constant while the kernel runs, h is not.
+  __device__ __forceinline__ void load(Columns<NT, FINE>& c, int j) const {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const uint4* p = reinterpret_cast<const uint4*>(q[n]);
-      const uint4 u = FINE ? p[0] : __ldg(p), v = FINE ? p[1] : __ldg(p + 1);
-      c.b[n][0] = make_uint2(u.x, u.y);
-      c.b[n][1] = make_uint2(u.z, u.w);
-      c.b[n][2] = make_uint2(v.x, v.y);
-      c.b[n][3] = make_uint2(v.z, v.w);
+      const uint4* p = reinterpret_cast<const uint4*>(q[n]) + j;
+      const uint4 u = FINE ? *p : __ldg(p);
+      c.b[n][2 * j] = make_uint2(u.x, u.y);
+      c.b[n][2 * j + 1] = make_uint2(u.z, u.w);
+    }
+  }
+  __device__ __forceinline__ void load_scales(Columns<NT, FINE>& c) const {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
       if constexpr (FINE) {
         const float4 f = *reinterpret_cast<const float4*>(s[n]);
         c.s[n][0] = f.x;
@@ -391,115 +366,109 @@ struct Places {
   }
 };
 
-// An up task of up to 4 NT rows: 32 columns of h and their planes.
-template <int G, int NT, typename S>
-__device__ __forceinline__ void up_task(const LayerArgs& a, Shared& s, S& st, const Task& k) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, log_p = s.plan.log_p;
-  const uint32_t flip = flip_register();
-  Places<NT, false> at;
-  at.at(a.xq, a.xs, a.H / kTileK, k.k0, s, k.block, false);
-  Columns<NT, false> x, ahead;  // one K position ahead: from the L2 they take longer than a step's products
-  at.load(ahead);
+// A consumer warp's part of a unit of up to 4 NT rows, its sums left in `part` ([n][tiles 0 1, tiles 2 3][lane][tile, 8 i]:
+// row 8 i + g of the tile, token 4n + t).
+template <int G, int NT, bool UP, typename S, typename Wait>
+__device__ __forceinline__ bool consume(const LayerArgs& a, Shared& s, S& st, const Unit& u, const Span& w, float* part,
+                                        const Wait& free_part) {
+  const int lane = threadIdx.x & 31, g = lane >> 2;
+  const uint32_t flip = flip_register(), two = two_register();
   float acc[4][NT][2] = {};
+  if (row_group(s, u, threadIdx.x / 32) < row_groups(a, u)) {
+    Places<NT, !UP> at;
+    at.at(UP ? a.xq : a.hq, UP ? a.xs : a.hs, (UP ? a.H : a.I) / kTileK, w.k0, s, u.block, !UP);
+    Columns<NT, !UP> x;
+    at.load(x, 0);
+    at.load(x, 1);
+    at.load_scales(x);
+    auto keep = [](int) {};
+    // the last tile's product is followed word by word by the loads of the next K position's columns: no registers of
+    // their own, and their latency passes under the next wait and the first tile
+    auto reload = [&](int j) { at.load(x, j); };
 #pragma unroll 1
-  for (int left = k.tiles; left > 0; --left) {
-    x = ahead;
-    if (left > 1) at.advance();  // the last one is read twice
-    at.load(ahead);
-    st.ring.wait(&s.abort);
-    const uint32_t words = st.ring.got + 16 * lane, scales = st.ring.got + 4 * g;
-    tile_product<G, NT, false, 0>(words, scales, x, flip, acc[0]);
-    tile_product<G, NT, false, tile_bytes(G)>(words, scales, x, flip, acc[1]);
-    tile_product<G, NT, false, 2 * tile_bytes(G)>(words, scales, x, flip, acc[2]);
-    tile_product<G, NT, false, 3 * tile_bytes(G)>(words, scales, x, flip, acc[3]);
-    st.ring.release();
-    st.fill(a, s);
-  }
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    // linear tiles, silu tiles: [tile][8 i + g] of token 4n + t
-    float v[8] = {acc[0][n][0], acc[0][n][1], acc[1][n][0], acc[1][n][1],
-                  acc[2][n][0], acc[2][n][1], acc[3][n][0], acc[3][n][1]};
-    if (!join(s, log_p, v)) continue;
-    float h[4], m = 0.0f;  // columns 8 i + g of the task's 32
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      h[i] = swiglu(v[4 + i], v[i]);
-      m = fmaxf(m, fabsf(h[i]));
-      bad |= !(fabsf(h[i]) <= 3.402823466e38f);
-    }
-    if (bad) m = INFINITY;
-#pragma unroll
-    for (int d = 16; d >= 4; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const bool finite = m <= 3.402823466e38f;
-    const int e = plane_exponent(m), r = 4 * n + t;
-    if (r < block_rows_of(k.block)) {
-      const size_t pair = s.pairs[block_pos(k.block) + r];
-      // column 8 i + g of these 32: eight i, element g, which is byte g / 4 + g % 4 * 2 of its eight
-      uint8_t* dst = a.hq + (pair * (a.I / kTileK) + k.row / 4) * kPlaneTile + k.row % 4 * 8 + (g >> 2) + (g & 3) * 2;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int q = finite ? plane_int(h[i], e) : 0;
-        dst[32 * i] = (uint8_t)((q + 128) >> 8);
-        dst[32 * i + 128] = (uint8_t)q;
-      }
-      if (g == 0) a.hs[pair * (a.I / 32) + k.row] = finite ? exp2_int(e) * 0.0625f : NAN;
-    }
-  }
-}
-
-// A down task of up to 4 NT rows: 32 outputs of each pair, weighted.
-template <int G, int NT, typename S>
-__device__ __forceinline__ void down_task(const LayerArgs& a, Shared& s, S& st, const Task& k) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, log_p = s.plan.log_p;
-  const uint32_t flip = flip_register();
-  Places<NT, true> at;
-  at.at(a.hq, a.hs, a.I / kTileK, k.k0, s, k.block, true);
-  Columns<NT, true> x, ahead;
-  at.load(ahead);
-  float acc[2][NT][2] = {};
-  uint32_t slot = 0;
-#pragma unroll 1
-  for (int i = 0; i < k.tiles; ++i) {
-    x = ahead;
-    if (i + 1 < k.tiles) at.advance();
-    at.load(ahead);
-    if (i % 2 == 0) {
+    for (int left = w.steps; left > 0; --left) {
+      if (left > 1) at.advance();  // the last one is read twice
       st.ring.wait(&s.abort);
-      slot = st.ring.got;
-    } else {
-      slot += tile_bytes(G);
-    }
-    const uint32_t words = slot + 16 * lane, scales = slot + 4 * g;
-    tile_product<G, NT, true, 0>(words, scales, x, flip, acc[0]);
-    tile_product<G, NT, true, 2 * tile_bytes(G)>(words, scales, x, flip, acc[1]);
-    if (i % 2 == 1 || i + 1 == k.tiles) {
+      const uint32_t words = st.ring.got + 16 * lane, scales = st.ring.got + 4 * g;
+      tile_product<G, NT, !UP, 0>(words, scales, x, flip, two, acc[0], keep);
+      tile_product<G, NT, !UP, tile_bytes(G)>(words, scales, x, flip, two, acc[1], keep);
+      tile_product<G, NT, !UP, 2 * tile_bytes(G)>(words, scales, x, flip, two, acc[2], keep);
+      tile_product<G, NT, !UP, 3 * tile_bytes(G)>(words, scales, x, flip, two, acc[3], reload);
+      at.load_scales(x);
       st.ring.release();
       st.fill(a, s);
     }
   }
-  // [tile][8 i + g] of tokens 4n + t
-  float v[8] = {acc[0][0][0], acc[0][0][1], acc[1][0][0], acc[1][0][1],
-                acc[0][NT - 1][0], acc[0][NT - 1][1], acc[1][NT - 1][0], acc[1][NT - 1][1]};
-  if (!join(s, log_p, v)) return;
+  if (!free_part()) return false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int r = 4 * n + t;
-    if (r < block_rows_of(k.block)) {
-      const int pair = s.pairs[block_pos(k.block) + r];
-      const float w = a.topk_w[pair];
-      float* dst = a.pair_out + (size_t)pair * a.H + k.row * kSpan + g;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) dst[8 * i] = v[4 * n + i] * w;
-    }
+    float4* p = reinterpret_cast<float4*>(part + n * 256 + lane * 4);
+    p[0] = make_float4(acc[0][n][0], acc[0][n][1], acc[1][n][0], acc[1][n][1]);
+    p[32] = make_float4(acc[2][n][0], acc[2][n][1], acc[3][n][0], acc[3][n][1]);
   }
+  return true;
 }
 
-// Four outputs per lane: the sum of a token's local pairs in slot order.
+// The finishers: 8 values of a lane for token row 4n + t of row group `group`, summed over the K groups in order.
+__device__ __forceinline__ void sum_parts(const float* part, int kw, int n, float (&v)[8]) {
+  const float4* p = reinterpret_cast<const float4*>(part + n * 256 + (threadIdx.x & 31) * 4);
+  float4 lo = p[0], hi = p[32];
+#pragma unroll 4
+  for (int k = 1; k < kw; ++k) {
+    const float4 l = p[k * (kPart / 4)], h = p[k * (kPart / 4) + 32];
+    lo = make_float4(lo.x + l.x, lo.y + l.y, lo.z + l.z, lo.w + l.w);
+    hi = make_float4(hi.x + h.x, hi.y + h.y, hi.z + h.z, hi.w + h.w);
+  }
+  v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+  v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+}
+
+// 32 columns of h: v holds the linear tiles, then the silu tiles.
+__device__ __forceinline__ void finish_up(const LayerArgs& a, const Shared& s, uint32_t block, int n, uint32_t group,
+                                          const float (&v)[8]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float h[4], m = 0.0f;  // columns 8 i + g
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[i] = swiglu(v[4 + i], v[i]);
+    m = fmaxf(m, fabsf(h[i]));
+    bad |= !(fabsf(h[i]) <= 3.402823466e38f);
+  }
+  if (bad) m = INFINITY;
+#pragma unroll
+  for (int d = 16; d >= 4; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  const bool finite = m <= 3.402823466e38f;
+  const int e = plane_exponent(m), r = 4 * n + t;
+  if (r >= block_rows_of(block)) return;
+  const size_t pair = s.pairs[block_pos(block) + r];
+  // column 8 i + g of these 32: eight i, element g, which is byte g / 4 + g % 4 * 2 of its eight
+  uint8_t* dst = a.hq + (pair * (a.I / kTileK) + group / 4) * kPlaneTile + group % 4 * 8 + (g >> 2) + (g & 3) * 2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int q = finite ? plane_int(h[i], e) : 0;
+    dst[32 * i] = (uint8_t)((q + 128) >> 8);
+    dst[32 * i + 128] = (uint8_t)q;
+  }
+  if (g == 0) a.hs[pair * (a.I / 32) + group] = finite ? exp2_int(e) * 0.0625f : NAN;
+}
+
+// 64 outputs of each pair, weighted.
+__device__ __forceinline__ void finish_down(const LayerArgs& a, const Shared& s, uint32_t block, int n, uint32_t group,
+                                            const float (&v)[8]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, r = 4 * n + t;
+  if (r >= block_rows_of(block)) return;
+  const int at = block_pos(block) + r;
+  const float w = s.pair_w[at];
+  float* dst = a.pair_out + (size_t)s.pairs[at] * a.H + group * kDownSpan + g;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) dst[8 * i] = v[i] * w;
+}
+
+// Four outputs per thread: the sum of a token's local pairs in slot order.
 template <typename A>
-__device__ __forceinline__ void combine(const LayerArgs& a, uint32_t task) {
-  const long at = (long)task * kCombine + 4 * (threadIdx.x & 31);
+__device__ __forceinline__ void combine(const LayerArgs& a, uint32_t unit) {
+  const long at = (long)unit * kCombine + 4 * threadIdx.x;
   if (at >= (long)a.T * a.H) return;
   const int t = (int)(at / a.H), n = (int)(at % a.H);
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -524,85 +493,174 @@ __global__ void __launch_bounds__(kThreads, 1) layer_kernel(const __grid_constan
   Shared& s = *reinterpret_cast<Shared*>(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < kStreamWarps * kMaxDepth) mbar_init(&s.ring_full[0][0] + threadIdx.x, 1);
-  if (threadIdx.x == 0) s.abort = 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kQueue; ++i) {
+      mbar_init(&s.known[i], 1);
+      mbar_init(&s.go[i], 1);
+      mbar_init(&s.done[i], kStreamWarps + kFinishers);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.part_full[i], kStreamWarps);
+      mbar_init(&s.part_empty[i], kFinishers);
+    }
+    s.abort = 0;
+  }
   fence_barrier_init();
   pdl_wait();
   pdl_trigger();
   build_lists(a, s);  // synchronises the CTA
-  if (threadIdx.x == 0) {
-    const Plan p = make_plan(a, s);
-    s.plan = p;
-    const int groups = kStreamWarps >> p.log_p;
-    const uint32_t base = atomicAdd(&a.counters->ticket, (uint32_t)groups);
-    for (int i = 0; i < groups; ++i) s.tickets[i][0] = base + i;
+  if (threadIdx.x < 2) {
+    // Longer runs along K per warp where that still leaves four units per SM (T = 64, a quarter of the experts: 166 us with
+    // the shorter ones, 157 with the longer), shorter ones otherwise (T = 1, H 2048, I 768: 23 us, 29 with the longer).
+    const int* kw = threadIdx.x ? a.kw2 : a.kw1;
+    const int groups = threadIdx.x ? a.H / kDownSpan : a.I / kUpSpan, mw = kStreamWarps / kw[1];
+    (threadIdx.x ? s.kw2 : s.kw1) = s.n_blocks * ((groups + mw - 1) / mw) >= 4 * (int)gridDim.x ? kw[1] : kw[0];
   }
   __syncthreads();
-  const int log_p = s.plan.log_p, group = warp >> log_p;
-  const bool leads = (warp & ((1 << log_p) - 1)) == 0 && lane == 0;  // takes the group's tickets, reports its work
-  Stream<G1, G2> st;
-  st.ring.init(smem_u32(smem + kFixedSmem) + warp * a.depth * kSlot, smem_u32(s.ring_full[warp]), kSlot, a.depth);
-  st.left = 0;
-  st.task = 0;
-  st.known = 1;
-  st.fill_slow(a, s);
-  if (threadIdx.x == 0) {  // the groups' second tickets, while the first tiles are on their way
-    const int groups = kStreamWarps >> log_p;
-    const uint32_t base = atomicAdd(&a.counters->ticket, (uint32_t)groups);
-    for (int i = 0; i < groups; ++i) s.tickets[i][1] = base + i;
-  }
-  __syncthreads();
-  st.known = 2;
-  st.fill_slow(a, s);
-  int ready = -1;
-  bool all_done = false;
-  // lane 0 waits for *c >= need, the warp follows
-  auto wait_for = [&](const uint32_t* c, uint32_t need) {
-    if (lane == 0 && load_acquire(c) < need) {
-      const uint64_t t0 = globaltimer_ns();
-      for (uint32_t it = 1; load_acquire(c) < need; ++it) {
-        if (*(volatile int*)&s.abort) break;
-        if ((it & 15u) == 0 && globaltimer_ns() - t0 > a.wait_ns) {
-          *(volatile int*)&s.abort = 1;
+  float* parts = reinterpret_cast<float*>(smem + kFixedSmem);
+  constexpr int kParts = kStreamWarps * kPart;  // floats of a unit's partial sums
+  volatile int* abort = &s.abort;
+  // a wait that gives up, its own limit run out or another's, ends the role; the call is reported as failed
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, kWaitBudgetNs));
+    if (!ok) *abort = 1;
+    return ok;
+  };
+
+  if (warp >= kStreamWarps)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
+  else
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
+  if (warp >= kStreamWarps + kFinishers) {
+    if (warp == kStreamWarps + kFinishers && lane == 0) {
+      const uint32_t mw1 = kStreamWarps / s.kw1, mw2 = kStreamWarps / s.kw2;
+      const uint32_t per_up = (a.I / kUpSpan + mw1 - 1) / mw1, per_down = (a.H / kDownSpan + mw2 - 1) / mw2;
+      const uint32_t n_up = s.n_blocks * per_up, n_down = s.n_blocks * per_down;
+      const uint32_t n_all = n_up + n_down + (uint32_t)(((long)a.T * a.H + kCombine - 1) / kCombine);
+      auto wait_for = [&](const uint32_t* c, uint32_t need) {  // *c >= need: other CTAs' finishers bring it about
+        const uint64_t t0 = globaltimer_ns();
+        for (uint32_t it = 1; load_acquire(c) < need; ++it) {
+          if (*abort) break;
+          if ((it & 15u) == 0 && globaltimer_ns() - t0 > a.wait_ns) {
+            *abort = 1;
+            break;
+          }
+        }
+      };
+      int ready = -1;
+      bool all_done = false;
+      uint32_t next = atomicAdd(&a.counters->ticket, 1u);
+      for (uint32_t seq = 0;; ++seq) {
+        const uint32_t ticket = next;
+        if (ticket < n_all) next = atomicAdd(&a.counters->ticket, 1u);  // under way while this one is queued
+        const int slot = seq % kQueue;
+        Unit u = {0, 0};
+        if (ticket < n_up + n_down) {
+          const bool up = ticket < n_up;
+          const uint32_t at = up ? ticket : ticket - n_up, per = up ? per_up : per_down, b = at / per;
+          const uint32_t block = s.block[b];
+          u.block = block | (up ? kUp : kDown) << 28;
+          u.row = at - b * per;
+        } else if (ticket < n_all) {
+          u.block = kSum << 28;
+          u.row = ticket - n_up - n_down;
+        }
+        if (!mbar_wait(&s.done[slot], (seq / kQueue & 1) ^ 1, abort, kWaitBudgetNs)) {
+          *abort = 1;
           break;
         }
+        s.unit[slot] = u;
+        mbar_arrive(&s.known[slot]);
+        const int kind = kind_of(u), e = block_expert(u.block);
+        if (kind == kDown && e != ready) {
+          wait_for(&a.counters->ready[e], (uint32_t)((__popcll(s.mask[e]) + kRows - 1) / kRows) * per_up * kFinishers + a.extra);
+          ready = e;
+        }
+        if (kind == kSum && !all_done) {
+          wait_for(&a.counters->done, n_down * kFinishers + a.extra);
+          all_done = true;
+        }
+        if (*abort) break;
+        mbar_arrive(&s.go[slot]);
+        if (kind == kStop) break;
       }
     }
-    __syncwarp();
-  };
-  for (uint32_t n = 0;; ++n) {
-    const uint32_t ticket = s.tickets[group][n % 4];
-    if (ticket >= s.plan.n_all) break;
-    uint32_t next = 0;
-    if (leads) next = atomicAdd(&a.counters->ticket, 1u);  // under way while the task runs
-    uint32_t* report = nullptr;
-    if (ticket < s.plan.n_up) {
-      const Task k = decode_task<G1, G2>(a, s, ticket);
-      report = &a.counters->ready[block_expert(k.block)];
-      if (block_rows_of(k.block) <= 4) up_task<G1, 1>(a, s, st, k);
-      else up_task<G1, 2>(a, s, st, k);
-    } else if (ticket < s.plan.n_up + s.plan.n_down) {
-      const Task k = decode_task<G1, G2>(a, s, ticket);
-      const int e = block_expert(k.block);
-      if (e != ready)
-        wait_for(&a.counters->ready[e], (uint32_t)((__popcll(s.mask[e]) + kRows - 1) / kRows) * s.plan.up_rows + a.extra);
-      ready = e;
-      report = &a.counters->done;
-      if (block_rows_of(k.block) <= 4) down_task<G2, 1>(a, s, st, k);
-      else down_task<G2, 2>(a, s, st, k);
-    } else {
-      if (!all_done) wait_for(&a.counters->done, s.plan.n_down + a.extra);
-      all_done = true;
-      combine<A>(a, ((ticket - s.plan.n_up - s.plan.n_down) << log_p) + (warp & ((1 << log_p) - 1)));
+  } else if (warp >= kStreamWarps) {
+    uint32_t n = 0, downs = 0;  // units with sums so far; down units finished and not reported
+    for (uint32_t seq = 0;; ++seq) {
+      const int slot = seq % kQueue;
+      if (!wait(&s.known[slot], seq / kQueue & 1)) break;
+      const Unit u = s.unit[slot];
+      const int kind = kind_of(u);
+      if (kind == kUp || kind == kDown) {
+        const int b = n & 1, kw = kind == kUp ? s.kw1 : s.kw2;
+        const int tokens = block_rows_of(u.block) <= 4 ? 1 : 2, works = kStreamWarps / kw * tokens;
+        if (!wait(&s.part_full[b], n / 2 & 1)) break;
+        for (int i = warp - kStreamWarps; i < works; i += kFinishers) {
+          const int mg = i / tokens, k = i % tokens;
+          const uint32_t group = u.row * (kStreamWarps / kw) + mg;
+          if (group >= row_groups(a, u)) break;
+          float v[8];
+          sum_parts(parts + b * kParts + mg * kw * kPart, kw, k, v);
+          if (kind == kUp) finish_up(a, s, u.block, k, group, v);
+          else finish_down(a, s, u.block, k, group, v);
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s.part_empty[b]);
+          if (kind == kUp) add_release(&a.counters->ready[block_expert(u.block)], 1u);
+        }
+        downs += kind == kDown;
+        ++n;
+      } else if (downs > 0) {  // only now: each report waits for the stores before it
+        if (lane == 0) add_release(&a.counters->done, downs);
+        downs = 0;
+      }
+      if (kind == kStop) break;
+      if (lane == 0) mbar_arrive(&s.done[slot]);
     }
-    if (leads) s.tickets[group][(n + 2) % 4] = next;
-    group_sync(log_p);
-    st.known = n + 3;
-    if (leads && report) add_release(report, 1u);  // the first warp's stores are all the task's
-    st.fill_slow(a, s);
+  } else {
+    const Span up = span_of(a, s, true), down = span_of(a, s, false);
+    Stream<G1, G2> st;
+    st.ring.init(smem_u32(parts + 2 * kParts) + warp * a.depth * kSlot, smem_u32(s.ring_full[warp]), kSlot, a.depth);
+    st.left = 0;
+    st.seq = 0;
+    st.more = true;
+    uint32_t n = 0;
+    for (uint32_t seq = 0;; ++seq) {
+      const int slot = seq % kQueue;
+      if (!wait(&s.known[slot], seq / kQueue & 1)) break;
+      st.fill(a, s);
+      if (!wait(&s.go[slot], seq / kQueue & 1)) break;
+      const Unit u = s.unit[slot];
+      const int kind = kind_of(u);
+      if (kind == kStop) break;
+      if (kind == kSum) {
+        combine<A>(a, u.row);
+      } else {
+        const int b = n & 1;
+        const uint32_t parity = (n / 2 & 1) ^ 1;
+        float* part = parts + b * kParts + warp * kPart;
+        auto free_part = [&] { return wait(&s.part_empty[b], parity); };
+        bool ok;
+        if (kind == kUp) {
+          if (block_rows_of(u.block) <= 4) ok = consume<G1, 1, true>(a, s, st, u, up, part, free_part);
+          else ok = consume<G1, 2, true>(a, s, st, u, up, part, free_part);
+        } else {
+          if (block_rows_of(u.block) <= 4) ok = consume<G2, 1, false>(a, s, st, u, down, part, free_part);
+          else ok = consume<G2, 2, false>(a, s, st, u, down, part, free_part);
+        }
+        if (!ok) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.part_full[b]);
+        ++n;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.done[slot]);
+    }
+    if (!st.ring.drain(a.depth) && lane == 0) atomicOr(&a.counters->status, kStatusTimeoutDrain);
   }
-  const bool drained = st.ring.drain();
   __syncthreads();
-  if (lane == 0 && !drained) atomicOr(&a.counters->status, kStatusTimeoutDrain);
   if (threadIdx.x == 0 && s.abort) atomicOr(&a.counters->status, kStatusTimeoutEpilogue);
   __syncthreads();
   if (threadIdx.x == 0) forward_status_to_sink(&a.counters->status, a.sink);
@@ -623,21 +681,45 @@ struct MoeArgs {
 
 constexpr int kSmemMax = 227 * 1024;
 
+// Consumer warps along K: the largest power of two that leaves each `least` steps and whose rounds over K waste no more
+// than one step in eight.
+int k_groups(int k_tiles, int least) {
+  for (int kw = kStreamWarps; kw > 1; kw /= 2)
+    if (k_tiles >= least * kw && 8 * kw * ((k_tiles + kw - 1) / kw) <= 9 * k_tiles + 4) return kw;
+  return 1;
+}
+
+// Packed matrices as a tensor [matrices][halves][row tiles][K positions x words], boxes [1][halves][rows][words].
+bool map_weights(CUtensorMap* map, const uint8_t* base, int k_tiles, int words, int row_tiles, int halves, int matrices,
+                 int rows) {
+  const uint64_t row = (uint64_t)k_tiles * words * 8;
+  const uint64_t dims[4] = {(uint64_t)k_tiles * words, (uint64_t)row_tiles, (uint64_t)halves, (uint64_t)matrices};
+  const uint64_t strides[3] = {row, row * row_tiles, row * row_tiles * halves};
+  const uint32_t box[4] = {(uint32_t)words, (uint32_t)rows, (uint32_t)halves, 1};
+  return encode_4d_words(map, base, dims, strides, box) == FBMOE_OK;
+}
+
 template <typename A, int G1, int G2>
 cudaError_t run_layer(const MoeArgs& m, const MoeLayout& L, int sms) {
   static DeviceFlags smem_set;
   cudaError_t e = set_max_dynamic_smem(layer_kernel<A, G1, G2>, kSmemMax, smem_set);
   if (e != cudaSuccess) return e;
-  LayerArgs a;
-  a.w1 = m.w1;
-  a.w2 = m.w2;
+  alignas(64) LayerArgs a;
+  if (!map_weights(&a.map1, m.w1, m.H / kTileK, tile_words(G1), m.I / kTileN, 2, m.E, 2) ||
+      !map_weights(&a.map2, m.w2, m.I / kTileK, tile_words(G2), m.H / kTileN, 1, m.E, 4))
+    return cudaErrorUnknown;
   a.T = m.T;
   a.H = m.H;
   a.I = m.I;
   a.E = m.E;
   a.offset = m.offset;
   constexpr int kSlot = step_bytes(G1 < G2 ? G1 : G2);
-  a.depth = (kSmemMax - (int)kFixedSmem) / (kStreamWarps * kSlot);
+  for (int i = 0; i < 2; ++i) {
+    a.kw1[i] = k_groups(m.H / kTileK, 2 + 2 * i);
+    a.kw2[i] = k_groups(m.I / kTileK, 2 + 2 * i);
+  }
+  constexpr int kFixed = (int)kFixedSmem + 2 * kStreamWarps * kPart * 4;
+  a.depth = (kSmemMax - kFixed) / (kStreamWarps * kSlot);
   if (a.depth > kMaxDepth) a.depth = kMaxDepth;
   a.topk_idx = reinterpret_cast<const int32_t*>(m.ws + L.topk_idx);
   a.topk_w = reinterpret_cast<const float*>(m.ws + L.topk_w);
@@ -652,7 +734,7 @@ cudaError_t run_layer(const MoeArgs& m, const MoeLayout& L, int sms) {
   const bool expire = test_expire_grid_wait();
   a.wait_ns = expire ? kTestGridWaitNs : kWaitBudgetNs;
   a.extra = expire ? 1u : 0u;
-  return launch_pdl(layer_kernel<A, G1, G2>, dim3(sms), dim3(kThreads), kFixedSmem + (size_t)a.depth * kStreamWarps * kSlot,
+  return launch_pdl(layer_kernel<A, G1, G2>, dim3(sms), dim3(kThreads), (size_t)kFixed + (size_t)a.depth * kStreamWarps * kSlot,
                     m.stream, a);
 }
 template <typename A, int G1>

@@ -36,8 +36,8 @@ __host__ __device__ constexpr int step_bytes(int group) { return kStepTiles * ti
 // ---------------------------------------------------------------- ring ------
 // One warp's ring.  Steps are issued and consumed in order.  Slots and barriers are shared-memory addresses.  Its waits
 // are for its own copies, which land by themselves; one that gives up all the same raises `abort` and closes the ring:
-// nothing more is issued, and the warp runs on over whatever the slots hold, to the end of its work, so that nothing
-// that counts on it is left waiting.  The caller reports the call as failed.
+// nothing more is issued, and the warp goes on over whatever the slots hold until it meets one of the waits that look at
+// `abort`.  The caller reports the call as failed.
 struct Ring {
   uint32_t begin, end, bars, put, put_bar, got, got_bar, parity;
   int slot_bytes, free;  // free: steps that may be issued (far below 0: closed)
@@ -50,18 +50,17 @@ struct Ring {
     end = slots + depth * bytes;
     parity = 0;
   }
-  // Issue one step: lane i < copies copies `bytes` from its `src` to the slot's offset i * stride.
-  __device__ __forceinline__ void issue(const uint8_t* src, int copies, uint32_t bytes, uint32_t stride) {
-    const int lane = threadIdx.x & 31;
-    if (lane < copies) {
-      if (lane == 0)
-        asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(put_bar),
-                     "r"(copies * bytes)
-                     : "memory");
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                       put + lane * stride),
-                   "l"(src), "r"(bytes), "r"(put_bar)
+  // Issue one step: the box of `map` at (x, row, half, matrix), `bytes` in all.
+  __device__ __forceinline__ void issue(const CUtensorMap* map, int x, int row, int half, int matrix, uint32_t bytes) {
+    if ((threadIdx.x & 31) == 0) {
+      asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(put_bar),
+                   "r"(bytes)
                    : "memory");
+      asm volatile(
+          "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+              put),
+          "l"(reinterpret_cast<uint64_t>(map)), "r"(put_bar), "r"(x), "r"(row), "r"(half), "r"(matrix)
+          : "memory");
     }
     --free;
     put += slot_bytes;
@@ -109,9 +108,17 @@ struct Ring {
       parity ^= 1;
     }
   }
-  // Before the CTA ends no copy may be under way.  All issued steps are consumed by then, unless the ring was closed:
-  // false, after one more limit's wait for the slot that did not come.
-  __device__ __forceinline__ bool drain() const { return free >= 0 || wait_slow(got_bar, parity); }
+  // Before the CTA ends no copy may be under way: those issued and not consumed are waited for (none after a complete
+  // call).  False when the limit runs out.
+  __device__ __forceinline__ bool drain(int depth) {
+    if (free < 0) return wait_slow(got_bar, parity);
+    bool ok = true;
+    while (free < depth) {
+      ok &= wait_slow(got_bar, parity);
+      release();
+    }
+    return ok;
+  }
 };
 
 // ---------------------------------------------------------------- planes ----
@@ -157,6 +164,17 @@ __device__ __forceinline__ uint32_t and_xor(uint32_t v, uint32_t flip) {
   asm("lop3.b32 %0, %1, 0xF0F0F0F0, %2, 0x6A;" : "=r"(r) : "r"(v), "r"(flip));
   return r;
 }
+// 2 v as a product: the shift would go to the logic pipe, which is the fuller one.
+__device__ __forceinline__ uint32_t twice(uint32_t v, uint32_t two) {
+  uint32_t r;
+  asm("mul.lo.u32 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(two));
+  return r;
+}
+__device__ __forceinline__ uint32_t two_register() {
+  uint32_t r;
+  asm volatile("mov.b32 %0, 2;" : "=r"(r));
+  return r;
+}
 __device__ __forceinline__ uint32_t flip_register() {
   uint32_t r;
   asm volatile("mov.b32 %0, 0x80808080;" : "=r"(r));
@@ -181,10 +199,10 @@ struct Columns {
 };
 
 // acc[n][i] (row g + 8 i of a tile, token 4n + t) += the tile at shared address words + AT (words = slot + 16 * lane,
-// scales = slot + 4 * g) times the columns.
-template <int G, int NT, bool FINE, int AT>
+// scales = slot + 4 * g) times the columns.  reload(j) is called once the columns' words 2j, 2j + 1 have been used.
+template <int G, int NT, bool FINE, int AT, typename Reload>
 __device__ __forceinline__ void tile_product(uint32_t words, uint32_t scales, const Columns<NT, FINE>& x, uint32_t flip,
-                                             float (&acc)[NT][2]) {
+                                             uint32_t two, float (&acc)[NT][2], const Reload& reload) {
   const uint4 lo = lds128<AT>(words), hi = lds128<AT + 512>(words);
   const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
   uint32_t sw[4];
@@ -195,26 +213,41 @@ __device__ __forceinline__ void tile_product(uint32_t words, uint32_t scales, co
     sw[3] = lds32<AT + kTileQ + 96>(scales);
   }
   int c[NT][4];
+  float part[NT][2];  // FINE: a weight group's sum
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const bool first = FINE || j * 32 % G == 0, last = FINE || (j + 1) * 32 % G == 0;
+    const bool first = j * 32 % G == 0, last = (j + 1) * 32 % G == 0;  // of the weight group
     const uint32_t el = and_xor(__funnelshift_l(wl[j], wl[j], 1), flip), eh = and_xor(__funnelshift_l(wh[j], wh[j], 1), flip);
     const uint32_t ol = and_xor(__funnelshift_r(wl[j], wl[j], 3), flip), oh = and_xor(__funnelshift_r(wh[j], wh[j], 3), flip);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      if (first)
+      if (FINE || first)
         mma_16832(c[n], el, eh, ol, oh, x.b[n][j].x, x.b[n][j].y, 0, 0, 0, 0);
       else
         mma_16832(c[n], el, eh, ol, oh, x.b[n][j].x, x.b[n][j].y, c[n][0], c[n][1], c[n][2], c[n][3]);
+    }
+    if (j % 2 == 1) reload(j / 2);
+    if (FINE) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float v = (float)(c[n][2 * i] * 256 + c[n][2 * i + 1]);
+          part[n][i] = first ? x.s[n][j] * v : fmaf(x.s[n][j], v, part[n][i]);
+        }
     }
     if (last) {
       const uint32_t s = sw[j * 32 / G];
       const float s0 = __uint_as_float(s << 16), s1 = __uint_as_float(s & 0xFFFF0000u);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float xs = x.s[n][FINE ? j : 0];
-        acc[n][0] = fmaf(s0 * xs, (float)(c[n][0] * 256 + c[n][1]), acc[n][0]);
-        acc[n][1] = fmaf(s1 * xs, (float)(c[n][2] * 256 + c[n][3]), acc[n][1]);
+        if (FINE) {
+          acc[n][0] = fmaf(s0, part[n][0], acc[n][0]);
+          acc[n][1] = fmaf(s1, part[n][1], acc[n][1]);
+        } else {
+          acc[n][0] = fmaf(s0 * x.s[n][0], (float)(c[n][0] * 256 + c[n][1]), acc[n][0]);
+          acc[n][1] = fmaf(s1 * x.s[n][0], (float)(c[n][2] * 256 + c[n][3]), acc[n][1]);
+        }
       }
     }
   }
