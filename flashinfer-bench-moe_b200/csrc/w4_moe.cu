@@ -272,11 +272,12 @@ struct Stream {
   int x, row, matrix;
   int left;        // steps of the unit being issued that are still to be issued
   uint32_t words;  // 8-byte elements of a tile
+  uint64_t policy;
   uint32_t seq;    // units begun
   bool more;
 
   __device__ __forceinline__ void step() {
-    ring.issue(map, x, row, 0, matrix, words * 32);
+    ring.issue(map, x, row, 0, matrix, words * 32, policy);
     x += words;
     --left;
   }
@@ -623,6 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1) layer_kernel(const __grid_constan
     const Span up = span_of(a, s, true), down = span_of(a, s, false);
     Stream<G1, G2> st;
     st.ring.init(smem_u32(parts + 2 * kParts) + warp * a.depth * kSlot, smem_u32(s.ring_full[warp]), kSlot, a.depth);
+    st.policy = l2_policy_evict_first();
     st.left = 0;
     st.seq = 0;
     st.more = true;

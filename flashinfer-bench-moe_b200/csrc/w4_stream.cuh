@@ -51,15 +51,15 @@ struct Ring {
     parity = 0;
   }
   // Issue one step: the box of `map` at (x, row, half, matrix), `bytes` in all.
-  __device__ __forceinline__ void issue(const CUtensorMap* map, int x, int row, int half, int matrix, uint32_t bytes) {
+  __device__ __forceinline__ void issue(const CUtensorMap* map, int x, int row, int half, int matrix, uint32_t bytes, uint64_t policy) {
     if ((threadIdx.x & 31) == 0) {
       asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(put_bar),
                    "r"(bytes)
                    : "memory");
       asm volatile(
-          "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
-              put),
-          "l"(reinterpret_cast<uint64_t>(map)), "r"(put_bar), "r"(x), "r"(row), "r"(half), "r"(matrix)
+          "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
+          "[%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(put),
+          "l"(reinterpret_cast<uint64_t>(map)), "r"(put_bar), "r"(x), "r"(row), "r"(half), "r"(matrix), "l"(policy)
           : "memory");
     }
     --free;

@@ -16,6 +16,7 @@ sys.path.insert(0, os.path.join(REPO, "tests"))
 import w4_oracle as W  # noqa: E402
 
 pytestmark = pytest.mark.gpu
+ROUTING_AT = 1280  # bytes of the layer's counters, rounded up: where its workspace holds the chosen experts
 BF16, F16, F32, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
 
 
@@ -426,3 +427,39 @@ def test_expired_wait_is_reported(fbmoe_lib):
         lib.fbmoe_test_expire_grid_wait(0)
     torch.cuda.synchronize()
     assert torch.equal(fbmoe_lib.forward_w4(*c.args(), sync_status=True), want)
+
+
+@pytest.mark.parametrize("kind", ["normal", "grid", "groups", "zero", "large", "nan", "inf"])
+def test_moe_routes_as_route(fbmoe_lib, kind):
+    """The layer's own routing, read back from its workspace, is fbmoe_route's bit for bit: ties at a group's or an
+    expert's boundary, equal values inside, values that are not numbers."""
+    lib = fbmoe_lib.load_library()
+    g = torch.Generator().manual_seed(11)
+    w1, w2 = random_packed(256, 128, 128, 1, (1,))[0], random_packed(128, 128, 128, 2, (1,))[0]
+    x = torch.zeros((64, 128), dtype=BF16, device="cuda")
+    for trial in range(30):
+        logits, bias = torch.randn((64, 256), generator=g), torch.randn(256, generator=g) * 0.1
+        if kind == "grid":
+            logits, bias = (logits * 2).round() / 2, (bias * 8).round() / 8
+        elif kind == "groups":   # equal groups, distinct experts in them
+            logits, bias = logits[:, :32].repeat(1, 8), bias[:32].repeat(8)
+        elif kind == "zero":
+            logits, bias = logits * 0, bias * (trial % 2)
+        elif kind == "large":
+            logits = logits * 60
+        elif kind == "nan":
+            logits[torch.rand(logits.shape, generator=g) < 0.02] = float("nan")
+        elif kind == "inf":
+            logits[torch.rand(logits.shape, generator=g) < 0.02] = float("inf")
+            logits[torch.rand(logits.shape, generator=g) < 0.02] = float("-inf")
+        logits, bias = logits.cuda(), bias.to(BF16).cuda()
+        idx, w = fbmoe_lib.route(logits, bias, 2.5)
+        n = lib.fbmoe_w4_workspace_size(64, 128, 128)
+        ws, out = torch.zeros(n, dtype=torch.uint8, device="cuda"), torch.empty_like(x)
+        assert lib.fbmoe_forward_w4(logits.data_ptr(), bias.data_ptr(), x.data_ptr(), 0, w1.data_ptr(), 128, w2.data_ptr(),
+                                    128, 64, 128, 128, 1, 0, 2.5, out.data_ptr(), ws.data_ptr(), n, None,
+                                    torch.cuda.current_stream().cuda_stream) == 0
+        at = ROUTING_AT
+        got_idx = ws[at:at + 2048].view(torch.int32).view(64, 8)
+        got_w = ws[at + 2048:at + 4096].view(torch.float32).view(64, 8)
+        assert torch.equal(got_idx, idx) and torch.equal(got_w.view(torch.int32), w.view(torch.int32))
