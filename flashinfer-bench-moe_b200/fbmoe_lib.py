@@ -452,30 +452,41 @@ def read_status(workspace: torch.Tensor) -> int:
 # ---------------------------------------------------------------- 4-bit weights with group scales
 # A packed matrix is a uint8 tensor [..., ceil(N / 16), K / 128, tile] (format: include/fbmoe.h); the tile's bytes tell
 # the group size.  These run on the tensors' own device and that device's current stream, and record no gradient.
+# Single-token calls take a few microseconds, so the checks are plain conditions and their messages are made on failure.
 W4_MAX_TOKENS = 64
 _W4_GROUPS = {1024 + 4096 // g: g for g in (32, 64, 128)}
 _W4_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
+_W4_X_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+_fns: Dict[str, object] = {}  # C entry points by name
 
 
-def _launch_on(dev: torch.device, fn, *args) -> None:
-    """Call a C entry point, its stream appended, with `dev` current."""
-    if dev.index == torch.cuda.current_device():
-        _check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+def _launch_on(index: int, name: str, *args) -> None:
+    """Call a C entry point, the current stream of device `index` appended, with that device current."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load_library(), name)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            _check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _check(rc)
 
 
 def _w4_shape(packed: torch.Tensor, name: str, n: int = None) -> Tuple[int, int, int]:
     """(N, K, group) of a packed tensor; n: the rows in use, all of the tiles' by default."""
-    _require(isinstance(packed, torch.Tensor) and packed.dtype == torch.uint8 and packed.dim() >= 3
-             and packed.is_contiguous() and packed.size(-1) in _W4_GROUPS and packed.size(-2) > 0
-             and packed.size(-3) > 0,
-             f"{name} must be a contiguous uint8 tensor [..., ceil(N / 16), K / 128, tile] as quantize_w4 packs it")
-    rows = packed.size(-3) * 16
-    n = rows if n is None else int(n)
-    _require(rows - 16 < n <= rows, f"n must be in {rows - 15}..{rows} for {name}'s {packed.size(-3)} row tiles")
-    return n, packed.size(-2) * 128, _W4_GROUPS[packed.size(-1)]
+    if not (isinstance(packed, torch.Tensor) and packed.dtype == torch.uint8 and packed.is_contiguous()):
+        raise RuntimeError(f"{name} must be a contiguous uint8 tensor as quantize_w4 packs it")
+    shape = packed.shape
+    if len(shape) < 3 or shape[-1] not in _W4_GROUPS or shape[-2] < 1 or shape[-3] < 1:
+        raise RuntimeError(f"{name} must be [..., ceil(N / 16), K / 128, tile] as quantize_w4 packs it, not {tuple(shape)}")
+    rows = shape[-3] * 16
+    if n is None:
+        n = rows
+    elif not rows - 16 < n <= rows:
+        raise RuntimeError(f"n must be in {rows - 15}..{rows} for {name}'s {shape[-3]} row tiles")
+    return int(n), shape[-2] * 128, _W4_GROUPS[shape[-1]]
 
 
 def quantize_w4(w: torch.Tensor, group_size: int = 128, scale: torch.Tensor = None,
@@ -490,9 +501,9 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, scale: torch.Tensor = No
     _require(isinstance(w, torch.Tensor) and w.dtype in _W4_TYPES, "w must be bfloat16, float16, float32 or float8_e4m3fn")
     _require(w.dim() >= 2 and w.is_contiguous(), "w must be contiguous [..., N, K]")
     _require(group_size in (32, 64, 128), "group_size must be 32, 64 or 128")
-    N, K = w.size(-2), w.size(-1)
+    shape = tuple(w.shape)
+    lead, N, K = shape[:-2], shape[-2], shape[-1]
     _require(N > 0 and K > 0 and K % 128 == 0, "K must be a positive multiple of 128 and N positive")
-    lead = tuple(w.shape[:-2])
     _require((block_scale is not None) == (w.dtype == torch.float8_e4m3fn),
              "block_scale goes with float8_e4m3fn weights, and only with them")
     if block_scale is not None:
@@ -507,7 +518,7 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, scale: torch.Tensor = No
     packed = torch.empty(lead + ((N + 15) // 16, K // 128, 1024 + 4096 // group_size), dtype=torch.uint8,
                          device=w.device)
     if packed.numel():
-        _launch_on(w.device, load_library().fbmoe_quantize_w4, w.data_ptr(), _W4_TYPES[w.dtype],
+        _launch_on(w.get_device(), "fbmoe_quantize_w4", w.data_ptr(), _W4_TYPES[w.dtype],
                    block_scale.data_ptr() if block_scale is not None else None,
                    scale.data_ptr() if scale is not None else None, w.numel() // (N * K), N, K, group_size,
                    packed.data_ptr())
@@ -520,10 +531,10 @@ def dequantize_w4(packed: torch.Tensor, n: int = None, dtype: torch.dtype = torc
     n, K, group = _w4_shape(packed, "packed", n)
     _require(dtype in _W4_TYPES and dtype != torch.float8_e4m3fn, "dtype must be bfloat16, float16 or float32")
     _require(packed.is_cuda, "packed must be a CUDA tensor")
-    out = torch.empty(tuple(packed.shape[:-3]) + (n, K), dtype=dtype, device=packed.device)
+    out = torch.empty(packed.shape[:-3] + (n, K), dtype=dtype, device=packed.device)
     if out.numel():
-        _launch_on(packed.device, load_library().fbmoe_dequantize_w4, packed.data_ptr(), out.numel() // (n * K), n, K,
-                   group, _W4_TYPES[dtype], out.data_ptr())
+        _launch_on(packed.get_device(), "fbmoe_dequantize_w4", packed.data_ptr(), out.numel() // (n * K), n, K, group,
+                   _W4_TYPES[dtype], out.data_ptr())
     return out
 
 
@@ -533,31 +544,37 @@ def linear_w4(x: torch.Tensor, weight: torch.Tensor, n: int = None, out: torch.T
     on ``dequantize_w4(weight, n)``."""
     n, K, group = _w4_shape(weight, "weight", n)
     _require(weight.dim() == 3, "weight must be one packed matrix [ceil(N / 16), K / 128, tile]")
-    _require(isinstance(x, torch.Tensor) and x.dtype in (torch.bfloat16, torch.float16),
-             "x must be bfloat16 or float16")
-    _require(x.dim() == 2 and x.size(1) == K, f"x must be [T, {K}]")
-    T = x.size(0)
-    _require(T <= W4_MAX_TOKENS, f"linear_w4 takes at most {W4_MAX_TOKENS} tokens; use a GEMM on dequantize_w4(weight)")
-    x_stride = x.stride(0) if T > 1 else K
-    _require(x.stride(1) == 1 and x_stride >= K and x_stride % 8 == 0,
+    _require(isinstance(x, torch.Tensor) and x.dtype in _W4_X_TYPES, "x must be bfloat16 or float16")
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != K:
+        raise RuntimeError(f"x must be [T, {K}], not {tuple(shape)}")
+    T = shape[0]
+    _require(T <= W4_MAX_TOKENS, "linear_w4 takes at most 64 tokens; use a GEMM on dequantize_w4(weight)")
+    x_stride, inner = x.stride()
+    if T <= 1:
+        x_stride = K
+    _require(inner == 1 and x_stride >= K and x_stride % 8 == 0,
              "x's rows must be contiguous and a multiple of 8 elements apart")
-    _require(x.is_cuda and weight.is_cuda and x.device == weight.device, "x and weight must be on one CUDA device")
+    dev = x.get_device()
+    _require(dev >= 0 and dev == weight.get_device(), "x and weight must be on one CUDA device")
     if out is None:
         out = torch.empty((T, n), dtype=x.dtype, device=x.device)
+        out_stride = n
     else:
-        _require(out.dtype == x.dtype and tuple(out.shape) == (T, n) and out.device == x.device
+        _require(out.dtype == x.dtype and tuple(out.shape) == (T, n) and out.get_device() == dev
                  and out.stride(1) == 1 and (T <= 1 or out.stride(0) >= n),
                  "out must be [T, n] in x's type on x's device, its rows contiguous")
+        out_stride = out.stride(0) if T > 1 else n
     if T:
-        _launch_on(x.device, load_library().fbmoe_linear_w4, x.data_ptr(), x_stride, _W4_TYPES[x.dtype], T,
-                   weight.data_ptr(), n, K, group, out.data_ptr(), out.stride(0) if T > 1 else n)
+        _launch_on(dev, "fbmoe_linear_w4", x.data_ptr(), x_stride, _W4_X_TYPES[x.dtype], T, weight.data_ptr(), n, K,
+                   group, out.data_ptr(), out_stride)
     return out
 
 
-def _w4_sink(dev: torch.device):
+def _w4_sink(index: int):
     """(key, address) of the device's status sink for forward_w4: one pinned word that lives as long as the process.  A
     capture cannot allocate it; a graph captured before the device's first call reports no status."""
-    key = (dev.index, -1)
+    key = (index, -1)
     sink = _sinks.get(key)
     if sink is None:
         if torch.cuda.is_current_stream_capturing():
@@ -581,44 +598,44 @@ def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2
     check_status(), or for this call with ``sync_status`` (or FBMOE_SYNC_STATUS=1)."""
     N1, H, group1 = _w4_shape(gemm1_weights, "gemm1_weights")
     N2, I, group2 = _w4_shape(gemm2_weights, "gemm2_weights")
-    x = hidden_states
-    _require(gemm1_weights.dim() == 4 and gemm2_weights.dim() == 4 and gemm1_weights.size(0) == gemm2_weights.size(0)
-             and 1 <= gemm1_weights.size(0) <= E_GLOBAL,
+    x, shape1, shape2 = hidden_states, gemm1_weights.shape, gemm2_weights.shape
+    _require(len(shape1) == 4 and len(shape2) == 4 and shape1[0] == shape2[0] and 1 <= shape1[0] <= E_GLOBAL,
              "gemm1_weights and gemm2_weights must hold the same 1..256 packed matrices")
-    _require(N1 == 2 * I and N2 == H, f"gemm1_weights must be packed [2I, H] and gemm2_weights packed [H, I]; they are "
-                                      f"[{N1}, {H}] and [{N2}, {I}]")
-    _require(isinstance(x, torch.Tensor) and x.dtype in (torch.bfloat16, torch.float16) and x.dim() == 2
-             and x.size(1) == H and x.is_contiguous(), f"hidden_states must be contiguous bfloat16 or float16 [T, {H}]")
-    T, E = x.size(0), gemm1_weights.size(0)
-    _require(T <= W4_MAX_TOKENS, f"fused_moe_w4 takes at most {W4_MAX_TOKENS} tokens")
+    if N1 != 2 * I or N2 != H:
+        raise RuntimeError("gemm1_weights must be packed [2I, H] and gemm2_weights packed [H, I]; they are "
+                           f"[{N1}, {H}] and [{N2}, {I}]")
+    _require(isinstance(x, torch.Tensor) and x.dtype in _W4_X_TYPES and x.dim() == 2 and x.size(1) == H
+             and x.is_contiguous(), "hidden_states must be contiguous bfloat16 or float16 [T, H]")
+    T, E = x.size(0), shape1[0]
+    _require(T <= W4_MAX_TOKENS, "fused_moe_w4 takes at most 64 tokens")
     _require(isinstance(routing_logits, torch.Tensor) and routing_logits.dtype == torch.float32
-             and tuple(routing_logits.shape) == (T, E_GLOBAL) and routing_logits.is_contiguous(),
+             and routing_logits.shape == (T, E_GLOBAL) and routing_logits.is_contiguous(),
              "routing_logits must be contiguous float32 [T, 256]")
     _require(isinstance(routing_bias, torch.Tensor) and routing_bias.dtype == torch.bfloat16
              and routing_bias.numel() == E_GLOBAL and routing_bias.is_contiguous(),
              "routing_bias must be 256 contiguous bfloat16")
     offset = int(local_expert_offset)
     _require(0 <= offset < E_GLOBAL, "local_expert_offset must be in 0..255")
-    dev = x.device
-    _require(all(t.is_cuda and t.device == dev for t in (routing_logits, routing_bias, x, gemm1_weights, gemm2_weights)),
-             "all tensors must be on one CUDA device")
+    dev = x.get_device()
+    _require(dev >= 0 and dev == routing_logits.get_device() == routing_bias.get_device()
+             == gemm1_weights.get_device() == gemm2_weights.get_device(), "all tensors must be on one CUDA device")
     if out is None:
-        out = torch.empty((T, H), dtype=x.dtype, device=dev)
+        out = torch.empty((T, H), dtype=x.dtype, device=x.device)
     else:
-        _require(out.dtype == x.dtype and tuple(out.shape) == (T, H) and out.is_contiguous() and out.device == dev,
+        _require(out.dtype == x.dtype and out.shape == (T, H) and out.is_contiguous() and out.get_device() == dev,
                  "out must be contiguous [T, H] in hidden_states' type on its device")
     if T:
-        lib = load_library()
         key, sink = _w4_sink(dev)
         word = _take_sink(key)
         if word:
             raise DeviceStatusError(word, "reported by an earlier forward_w4 on this device")
-        ws = torch.empty(lib.fbmoe_w4_workspace_size(T, H, I), dtype=torch.uint8, device=dev)
-        _launch_on(dev, lib.fbmoe_forward_w4, routing_logits.data_ptr(), routing_bias.data_ptr(), x.data_ptr(),
-                   _W4_TYPES[x.dtype], gemm1_weights.data_ptr(), group1, gemm2_weights.data_ptr(), group2, T, H, I, E,
-                   offset, float(routed_scaling_factor), out.data_ptr(), ws.data_ptr(), ws.numel(), sink)
+        nbytes = load_library().fbmoe_w4_workspace_size(T, H, I)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _launch_on(dev, "fbmoe_forward_w4", routing_logits.data_ptr(), routing_bias.data_ptr(), x.data_ptr(),
+                   _W4_X_TYPES[x.dtype], gemm1_weights.data_ptr(), group1, gemm2_weights.data_ptr(), group2, T, H, I, E,
+                   offset, routed_scaling_factor, out.data_ptr(), ws.data_ptr(), nbytes, sink)
         if sync_status_default() if sync_status is None else sync_status:
-            torch.cuda.current_stream(dev).synchronize()
+            torch.cuda.current_stream(x.device).synchronize()
             word = _take_sink(key)
             if word:
                 raise DeviceStatusError(word, "reported by this forward_w4")

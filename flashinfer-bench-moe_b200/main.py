@@ -57,7 +57,6 @@ def fused_moe(
     )
 
 
-@torch.no_grad()
 def fused_moe_w4(
     routing_logits: torch.Tensor,
     routing_bias: torch.Tensor,
