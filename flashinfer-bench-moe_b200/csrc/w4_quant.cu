@@ -22,129 +22,181 @@ constexpr float kMinNormal = 1.17549435e-38f;
 
 enum Type { kBf16 = FBMOE_BF16, kF16 = FBMOE_F16, kF32 = FBMOE_F32, kE4m3 = FBMOE_E4M3 };
 
-// Eight consecutive weights as fp32.
+// Eight consecutive weights as they are held, and as fp32.
 template <int TYPE>
-__device__ __forceinline__ void load8(const void* base, size_t at, float (&v)[8]) {
-  if constexpr (TYPE == kBf16) {
-    const uint4 r = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + at));
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-    }
-  } else if constexpr (TYPE == kF16) {
-    const uint4 r = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + at));
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  } else if constexpr (TYPE == kF32) {
-    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at);
-    const float4 a = __ldg(p), b = __ldg(p + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint2 r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(base) + at));
-    const uint32_t w[2] = {r.x, r.y};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
-      const float2 f = __half22float2(__half2(h));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+struct Raw8 {
+  uint4 a, b;  // b: fp32 only
+  __device__ __forceinline__ void load(const void* base, size_t at) {
+    if constexpr (TYPE == kE4m3) {
+      const uint2 r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(base) + at));
+      a.x = r.x;
+      a.y = r.y;
+    } else if constexpr (TYPE == kF32) {
+      const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(base) + at);
+      a = __ldg(p);
+      b = __ldg(p + 1);
+    } else {
+      a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + at));
     }
   }
+  __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
+  // bs: the scale of an e4m3 block
+  __device__ __forceinline__ void widen(float (&v)[8], float bs) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    if constexpr (TYPE == kBf16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    } else if constexpr (TYPE == kF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    } else if constexpr (TYPE == kF32) {
+      const uint32_t u[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = __uint_as_float(w[i]);
+        v[4 + i] = __uint_as_float(u[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
+        const float2 f = __half22float2(__half2(h));
+        v[2 * i] = __fmul_rn(f.x, bs);
+        v[2 * i + 1] = __fmul_rn(f.y, bs);
+      }
+    }
+  }
+};
+
+// max(m, |v|), NaN if either is.
+__device__ __forceinline__ float max_abs_nan(float m, float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
-// rint(w / s) with the IEEE quotient, r = 1 / s: y = w * r is within 2 ulps of it, so only a y next to a half integer
-// needs the division itself.
-__device__ __forceinline__ int quotient(float w, float s, float r) {
-  const float y = w * r;
-  float n = rintf(y);
-  if (fabsf(y - n) > 0.499995f) n = rintf(__fdiv_rn(w, s));
-  return (int)fminf(fmaxf(n, -8.0f), 7.0f);
+// The word of eight weights v, s their scale, r = 1 / s: u = clamp(rint(v / s), -8, 7) + 8 with the IEEE quotient.
+// y = v * r is within 3 ulps of it, so only a y next to a half integer needs the division; y + 1.5 * 2^23 + 8 holds u in its
+// low bits.  CLAMP: the scale was given (one made from the largest |v| leaves |y| < 7.04).
+template <bool CLAMP>
+__device__ __forceinline__ uint32_t quantize8(const float (&v)[8], float s, float r) {
+  constexpr float kMagic = 12582912.0f;
+  const uint64_t rr = f32x2_pack(r, r), up = f32x2_pack(kMagic, kMagic), down = f32x2_pack(-kMagic, -kMagic),
+                 eight = f32x2_pack(8.0f, 8.0f), minus = f32x2_pack(-1.0f, -1.0f);
+  float off = 0.0f;  // largest distance of a y from its integer
+  uint32_t b[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint64_t y = f32x2_mul(f32x2_pack(v[2 * i], v[2 * i + 1]), rr);
+    if (CLAMP) {
+      float p, q;
+      f32x2_unpack(y, p, q);
+      y = f32x2_pack(fminf(fmaxf(p, -9.0f), 8.0f), fminf(fmaxf(q, -9.0f), 8.0f));
+    }
+    const uint64_t m = add2(y, up), n = add2(m, down);  // n = rint(y)
+    uint64_t d = y;
+    f32x2_fma(d, n, minus);
+    float p, q;
+    f32x2_unpack(d, p, q);
+    off = fmaxf(off, fmaxf(fabsf(p), fabsf(q)));
+    float lo, hi;
+    f32x2_unpack(add2(m, eight), lo, hi);
+    if (CLAMP) {
+      lo = fminf(fmaxf(lo, kMagic), kMagic + 15.0f);
+      hi = fminf(fmaxf(hi, kMagic), kMagic + 15.0f);
+    }
+    b[2 * i] = __float_as_uint(lo);
+    b[2 * i + 1] = __float_as_uint(hi);
+  }
+  if (off > 0.499995f) {  // rare, but common for ties of short weights
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float n = rintf(__fdiv_rn(v[i], s));
+      b[i] = __float_as_uint(fminf(fmaxf(n, -8.0f), 7.0f) + (kMagic + 8.0f));
+    }
+  }
+  // bytes of elements (0, 4, 1, 5) and (2, 6, 3, 7): the even and the odd nibbles
+  const uint32_t even = __byte_perm(__byte_perm(b[0], b[4], 0x0040), __byte_perm(b[1], b[5], 0x0040), 0x5410);
+  const uint32_t odd = __byte_perm(__byte_perm(b[2], b[6], 0x0040), __byte_perm(b[3], b[7], 0x0040), 0x5410);
+  const uint32_t u = (even & 0x0F0F0F0Fu) | ((odd & 0x0F0F0F0Fu) << 4);
+  return __funnelshift_l(u, u, 3);
 }
+// bf16(m / 7) with the IEEE quotient: m * RN(1 / 7) is within 2 ulps of it, which matters only next to the middle between
+// two bf16 numbers.
+__device__ __forceinline__ uint32_t scale_bits(float m) {
+  float q = m * (1.0f / 7.0f);
+  if ((__float_as_uint(q) & 0xFFFFu) - 0x7FFCu <= 8u) q = __fdiv_rn(m, 7.0f);
+  const uint32_t sb = __bfloat16_as_ushort(__float2bfloat16_rn(q));
+  return sb < 0x0080u ? 0u : sb;  // below the smallest normal number
+}
+constexpr uint32_t kZeroWord = 0x44444444u;  // rotl32(0x88888888, 3): q = 0
 
-template <int TYPE, int G>
-__global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const void* __restrict__ w,
+template <int TYPE, int G, bool GIVEN>
+__global__ void __launch_bounds__(kWarps * 32, TYPE == kF32 ? 2 : 3) quantize_kernel(const void* __restrict__ w,
                                                                const float* __restrict__ block_scale,
-                                                               const uint16_t* __restrict__ given, long tiles, int N,
+                                                               const uint16_t* __restrict__ given, uint32_t tiles, int N,
                                                                int K, uint8_t* __restrict__ packed) {
   constexpr int kGroups = 128 / G, kPer = G / 32;  // groups of a tile; words of a lane per group
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kt_n = K / kTileK, nt_n = (N + kTileN - 1) / kTileN;
+  const uint32_t kt_n = K / kTileK, nt_n = (N + kTileN - 1) / kTileN;
   pdl_wait();
   pdl_trigger();
-  for (long tile = (long)blockIdx.x * kWarps + (threadIdx.x >> 5); tile < tiles; tile += (long)gridDim.x * kWarps) {
-    const int kt = (int)(tile % kt_n);
-    const long b = tile / kt_n / nt_n;
-    const int nt = (int)(tile / kt_n % nt_n);
+  for (uint32_t tile = blockIdx.x * kWarps + (threadIdx.x >> 5); tile < tiles; tile += gridDim.x * kWarps) {
+    const uint32_t row_tile = tile / kt_n, kt = tile - row_tile * kt_n, b = row_tile / nt_n, nt = row_tile - b * nt_n;
     uint8_t* out = packed + (size_t)tile * tile_bytes(G);
     uint32_t scale_word[kGroups] = {};
-    float v[2][4][8];
+    Raw8<TYPE> raw[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int row = nt * kTileN + 8 * h + g;
       const size_t at = ((size_t)b * N + row) * K + (size_t)kt * kTileK + 8 * t;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (row < N) {
-          load8<TYPE>(w, at + 32 * j, v[h][j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[h][j][i] = 0.0f;
-        }
+        if (row < N) raw[h][j].load(w, at + 32 * j);
+        else raw[h][j].zero();
       }
     }
-    if (TYPE == kE4m3) {  // a tile lies inside one 128 x 128 block
-      const float bs = __ldg(block_scale + ((size_t)b * ((N + 127) / 128) + nt / 8) * kt_n + kt);
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[h][j][i] = __fmul_rn(v[h][j][i], bs);
-    }
+    // a tile lies inside one 128 x 128 block
+    const float bs = TYPE == kE4m3 ? __ldg(block_scale + ((size_t)b * ((N + 127) / 128) + nt / 8) * kt_n + kt) : 1.0f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int row = nt * kTileN + 8 * h + g;
       uint32_t word[4];
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr) {
-        float m = 0.0f;
-        bool bad = false;  // a NaN or an infinity
+        float v[kPer][8], m = 0.0f;
 #pragma unroll
-        for (int j = gr * kPer; j < (gr + 1) * kPer; ++j)
+        for (int j = 0; j < kPer; ++j) {
+          raw[h][gr * kPer + j].widen(v[j], bs);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            m = fmaxf(m, fabsf(v[h][j][i]));
-            bad |= !(fabsf(v[h][j][i]) <= 3.402823466e38f);
-          }
-        m = bad ? INFINITY : m;
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        uint32_t sb;
-        if (given != nullptr) {
-          sb = row < N ? given[((size_t)b * N + row) * (K / G) + (size_t)kt * kGroups + gr] : 0u;
-        } else {
-          sb = __bfloat16_as_ushort(__float2bfloat16_rn(__fdiv_rn(m, 7.0f)));
-          if (__uint_as_float(sb << 16) < kMinNormal) sb = 0u;
+          for (int i = 0; i < 8; ++i) m = max_abs_nan(m, v[j][i]);
         }
-        if (m == INFINITY) sb = 0x7FC0u;
-        const float s = __uint_as_float(sb << 16), r = __frcp_rn(s);
+        m = max_abs_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max_abs_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        uint32_t sb;
+        if (GIVEN)
+          sb = row < N ? given[((size_t)b * N + row) * (K / G) + (size_t)kt * kGroups + gr] : 0u;
+        else
+          sb = scale_bits(m);
+        if (!(m <= 3.402823466e38f)) sb = 0x7FC0u;  // an infinity or a NaN among them
+        const float s = __uint_as_float(sb << 16);
+        float r;
+        asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
         const bool use = s >= kMinNormal && s <= 3.402823466e38f;
 #pragma unroll
-        for (int j = gr * kPer; j < (gr + 1) * kPer; ++j) {
-          uint32_t u = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            u |= (uint32_t)((use ? quotient(v[h][j][i], s, r) : 0) + 8) << (4 * (i >> 1) + 16 * (i & 1));
-          word[j] = __funnelshift_l(u, u, 3);
-        }
+        for (int j = 0; j < kPer; ++j) word[gr * kPer + j] = use ? quantize8<GIVEN>(v[j], s, r) : kZeroWord;
         scale_word[gr] |= sb << (16 * h);
       }
       *reinterpret_cast<uint4*>(out + 512 * h + 16 * lane) = make_uint4(word[0], word[1], word[2], word[3]);
@@ -159,9 +211,14 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const void* __res
 template <int TYPE>
 __device__ __forceinline__ void store8(void* base, size_t at, const float (&v)[8]) {
   if constexpr (TYPE == kF32) {
-    float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + at);
-    p[0] = make_float4(v[0], v[1], v[2], v[3]);
-    p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    // Two lanes of a quad swap halves, so that a store writes whole 32-byte sectors: first the even lane's, then the odd's.
+    const bool odd = threadIdx.x & 1;
+    float o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __shfl_xor_sync(__activemask(), odd ? v[i] : v[4 + i], 1);
+    float* p = reinterpret_cast<float*>(base) + at - (odd ? 4 : 0);
+    *reinterpret_cast<float4*>(p) = odd ? make_float4(o[0], o[1], o[2], o[3]) : make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 8) = odd ? make_float4(v[4], v[5], v[6], v[7]) : make_float4(o[0], o[1], o[2], o[3]);
   } else {
     uint32_t w[4];
 #pragma unroll
@@ -179,16 +236,14 @@ __device__ __forceinline__ void store8(void* base, size_t at, const float (&v)[8
 }
 
 template <int TYPE, int G>
-__global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* __restrict__ packed, long tiles, int N,
+__global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* __restrict__ packed, uint32_t tiles, int N,
                                                                  int K, void* __restrict__ out) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kt_n = K / kTileK, nt_n = (N + kTileN - 1) / kTileN;
+  const uint32_t kt_n = K / kTileK, nt_n = (N + kTileN - 1) / kTileN;
   pdl_wait();
   pdl_trigger();
-  for (long tile = (long)blockIdx.x * kWarps + (threadIdx.x >> 5); tile < tiles; tile += (long)gridDim.x * kWarps) {
-    const int kt = (int)(tile % kt_n);
-    const long b = tile / kt_n / nt_n;
-    const int nt = (int)(tile / kt_n % nt_n);
+  for (uint32_t tile = blockIdx.x * kWarps + (threadIdx.x >> 5); tile < tiles; tile += gridDim.x * kWarps) {
+    const uint32_t row_tile = tile / kt_n, kt = tile - row_tile * kt_n, b = row_tile / nt_n, nt = row_tile - b * nt_n;
     const uint8_t* in = packed + (size_t)tile * tile_bytes(G);
     const uint4 q[2] = {__ldg(reinterpret_cast<const uint4*>(in + 16 * lane)),
                         __ldg(reinterpret_cast<const uint4*>(in + 512 + 16 * lane))};
@@ -229,8 +284,9 @@ unsigned grid_for(long tiles) {
 template <int TYPE, int G>
 cudaError_t run_quantize(const void* w, const float* bs, const void* given, long tiles, int N, int K, void* packed,
                          cudaStream_t stream) {
-  return launch_pdl(quantize_kernel<TYPE, G>, dim3(grid_for(tiles)), dim3(kWarps * 32), 0, stream, w, bs,
-                    reinterpret_cast<const uint16_t*>(given), tiles, N, K, reinterpret_cast<uint8_t*>(packed));
+  return launch_pdl(given ? quantize_kernel<TYPE, G, true> : quantize_kernel<TYPE, G, false>, dim3(grid_for(tiles)),
+                    dim3(kWarps * 32), 0, stream, w, bs, reinterpret_cast<const uint16_t*>(given), (uint32_t)tiles, N, K,
+                    reinterpret_cast<uint8_t*>(packed));
 }
 template <int TYPE>
 cudaError_t pick_quantize(int group, const void* w, const float* bs, const void* given, long tiles, int N, int K,
@@ -242,7 +298,7 @@ cudaError_t pick_quantize(int group, const void* w, const float* bs, const void*
 template <int TYPE, int G>
 cudaError_t run_dequantize(const void* packed, long tiles, int N, int K, void* out, cudaStream_t stream) {
   return launch_pdl(dequantize_kernel<TYPE, G>, dim3(grid_for(tiles)), dim3(kWarps * 32), 0, stream,
-                    reinterpret_cast<const uint8_t*>(packed), tiles, N, K, out);
+                    reinterpret_cast<const uint8_t*>(packed), (uint32_t)tiles, N, K, out);
 }
 template <int TYPE>
 cudaError_t pick_dequantize(int group, const void* packed, long tiles, int N, int K, void* out, cudaStream_t stream) {
@@ -272,6 +328,7 @@ extern "C" FBMOE_API int fbmoe_quantize_w4(const void* w, int w_type, const floa
   if (!w || !packed || (w_type == FBMOE_E4M3 && !block_scale)) return FBMOE_ERR_NULL_POINTER;
   if (w4::misaligned(w) || w4::misaligned(packed) || ((uintptr_t)block_scale & 3) || ((uintptr_t)scale_bf16 & 1))
     return FBMOE_ERR_MISALIGNED;
+  if (batch > INT64_C(0x7fffffff) / ((N - 1) / 16 + 1) / (K / 128)) return FBMOE_ERR_INVALID_ARG;  // 4e12 weights
   const long tiles = (long)batch * ((N - 1) / 16 + 1) * (K / 128);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   cudaError_t e;
@@ -291,6 +348,7 @@ extern "C" FBMOE_API int fbmoe_dequantize_w4(const void* packed, int64_t batch, 
   if (batch == 0) return FBMOE_OK;
   if (!packed || !out) return FBMOE_ERR_NULL_POINTER;
   if (w4::misaligned(packed) || w4::misaligned(out)) return FBMOE_ERR_MISALIGNED;
+  if (batch > INT64_C(0x7fffffff) / ((N - 1) / 16 + 1) / (K / 128)) return FBMOE_ERR_INVALID_ARG;  // 4e12 weights
   const long tiles = (long)batch * ((N - 1) / 16 + 1) * (K / 128);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   cudaError_t e;
