@@ -113,6 +113,19 @@ static int encode_2d(CUtensorMap* map, CUtensorMapDataType dtype, int elem_bytes
   return r == CUDA_SUCCESS ? FBMOE_OK : FBMOE_ERR_DRIVER;
 }
 
+int encode_strided_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t rows,
+                      uint64_t row_bytes, uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  if (!get_encode()) return FBMOE_ERR_DRIVER;
+  const cuuint64_t dims[2] = {inner, rows};
+  const cuuint64_t strides[1] = {row_bytes};
+  const cuuint32_t box[2] = {box_inner, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = g_encode(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FBMOE_OK : FBMOE_ERR_DRIVER;
+}
+
 int encode_4d_words(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
                     const uint32_t (&box)[4]) {
   if (!get_encode()) return FBMOE_ERR_DRIVER;

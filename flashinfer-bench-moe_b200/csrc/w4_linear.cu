@@ -1,8 +1,24 @@
 // w4_linear.cu -- products of a few tokens with a packed 4-bit matrix: out[t, n] = sum over k of x[t, k] q[n, k] s[n, k / G],
 // x and out bf16 or f16, sums in fp32, one rounding.
 //
-// One CTA per 16-row tile and block of up to 8 NT tokens; its eight warps take the tiles along K in turn and their
-// partial sums are added in warp order through shared memory.
+// tiles_kernel (few tokens and small matrices): one CTA per 16-row tile and block of up to 8 NT tokens; its eight warps take
+// the tiles along K in turn and their partial sums are added in warp order through shared memory.  Bound by latency.
+//
+// rows_kernel: 128 rows of the matrix are the M of a tcgen05 product, up to 64 tokens its N.  Per K position (128 columns)
+// one tensor copy brings the eight row tiles and two bring x; four warps decode, a thread per row, to exact 16-bit floats q
+// in tensor memory, the product's A operand; the tensor core sums each scale group into columns of its own (x and q exact,
+// sums fp32), and eight warps, a thread per row and half of the tokens, add s times that sum to totals in registers.  So no
+// weight is rounded and the matrix is read once for all tokens.  A cluster of S CTAs splits K where there are fewer blocks
+// of rows than half the SMs; their totals are added in rank order through shared memory.
+//
+// N = 18432, K = 7168, G = 128 on a B200: 23.6 us for 9 to 16 tokens, 24.7 for 32, 28.3 for 64 (reading alone 10.5 to 10.9),
+// tiles_kernel 30 to 99; G = 32: 27.5, 30.4, 45.8.  What it cost on the way, at 64 tokens: 50 us with the decoded tile in
+// shared memory (32 KB written and 32 KB read per position: 1350 cycles), 44 with it in tensor memory, 32.5 with two issuing
+// threads, one commit per position and two groups of decoders, 31.2 with lanes chosen by elect.sync, 28.4 with two groups of
+// totals (in turns by position in place of by tokens: 32.9).  Bound by the roles' waits on one another: a position takes 0.33 to
+// 0.42 us, and without the decoding it would take 20.3 us for one token (29.1 for 64, before the second group of totals),
+// without most of the products 23.4 (30.3), without the totals' sums 22.4 (25.2); four groups of decoders are no faster.
+#include <type_traits>
 #include "fbmoe.h"
 #include "fbmoe_launch.h"
 #include "w4_common.cuh"
@@ -14,7 +30,7 @@ namespace {
 constexpr int kWarps = 8;
 
 template <typename A, int G, int NT>
-__global__ void __launch_bounds__(kWarps * 32) linear_kernel(const typename A::Raw* __restrict__ x, long ldx, int T,
+__global__ void __launch_bounds__(kWarps * 32) tiles_kernel(const typename A::Raw* __restrict__ x, long ldx, int T,
                                                              const uint8_t* __restrict__ packed, int N, int K,
                                                              typename A::Raw* __restrict__ out, long ldo) {
   __shared__ float part[kWarps][NT * 128];
@@ -56,6 +72,384 @@ __global__ void __launch_bounds__(kWarps * 32) linear_kernel(const typename A::R
   }
 }
 
+// ---------------------------------------------------------------- rows_kernel
+constexpr int kM = 128;  // rows of the matrix per CTA
+// Groups of four warps that decode, taking turns at K positions; that add up, half of the tokens each; and threads that issue
+// products, taking turns at batches (below).
+constexpr int kDecoders = 2, kTotals = 2, kIssuers = 2;
+// Places in shared and tensor memory.  What is used in turns has a number of places that is a multiple of the users': a place
+// then always has the same one, whose phases follow one another.
+constexpr int kRawStages = 6, kXStages = 4;
+constexpr int kScaleSlots = 16;  // more than the decoders can be ahead of the totals (kDecoded + kSums, 12 at most)
+constexpr int kFirstTotals = 4, kFirstDecoder = kFirstTotals + 4 * kTotals;  // warps; 0 and 3 copy, 1 and 2 issue products
+constexpr int kRowsThreads = 32 * (kFirstDecoder + 4 * kDecoders);
+constexpr uint64_t kWaitBudgetNs = 4000000000ull;
+
+template <int G, int NP>
+struct RowsSmem {
+  static constexpr int kTile = tile_bytes(G), kRawTx = 8 * kTile, kRaw = (kRawTx + 127) / 128 * 128;
+  static constexpr int kX = NP * kTileK * 2;
+  static constexpr int kGroups = kTileK / G;
+  // Tensor memory: the first half holds group sums, the other decoded tiles of 64 columns (six of those were no faster).
+  static constexpr int kDecodedAt = 256, kDecoded = (512 - kDecodedAt) / 64;
+  static constexpr int kSumCols = NP < 32 ? 32 : NP, kSums = kDecodedAt / kSumCols;
+  // group sums per commit: a commit costs its thread 90 ns (measured), so as many as leave two places of that many
+  static constexpr int kBatch = kGroups < kSums / 2 ? kGroups : kSums / 2, kBatches = kGroups / kBatch;  // per K position
+  static constexpr int kPlaces = kSums / kBatch;
+  static_assert(kPlaces % kIssuers == 0 && kXStages % kIssuers == 0 && kDecoded % kIssuers == 0 && kDecoded % kDecoders == 0 &&
+                    kRawStages % kDecoders == 0 && kScaleSlots % kDecoders == 0 && kScaleSlots > kDecoded + kSums,
+                "see kRawStages");
+  static constexpr int x_at = 0;
+  static constexpr int raw_at = x_at + kXStages * kX;
+  static constexpr int scale_at = raw_at + kRawStages * kRaw;
+  static constexpr int bar_at = scale_at + kScaleSlots * kGroups * kM * 4;
+  static constexpr int used = bar_at + 640 + 1024;  // and the alignment of the first
+  // More than half of an SM's, so that no two share one: each takes all of its tensor memory, and CTAs of two clusters that
+  // waited for each other's would wait for good.
+  static constexpr int total = used > 116 * 1024 ? used : 116 * 1024;
+};
+
+__device__ __forceinline__ void swap(uint4& a, uint4& b) {
+  const uint4 c = a;
+  a = b;
+  b = c;
+}
+// One lane of a warp that has not diverged.  The compiler then keeps what is the same in all lanes in uniform registers, as
+// copies and products take it; a branch on the lane's number made the whole 1 to 2 us slower.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float load_cluster(uint32_t smem_addr, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
+// tmem_ld16_pairs of eight columns.
+__device__ __forceinline__ void tmem_ld8_pairs(uint32_t taddr, uint64_t (&v)[4]) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("mov.b64 %0, {%1, %2};" : "=l"(v[i]) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
+}
+// Box (0, 0, k, row tile) of a map of one matrix.
+__device__ __forceinline__ void load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int k, int tile, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
+      "[%0], [%1, {%3, %3, %4, %5}], [%2], %6;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(k), "r"(tile), "l"(policy)
+      : "memory");
+}
+
+template <typename A, int G, int NP>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+    rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, int T, int N, int kt_n,
+                int splits, typename A::Raw* __restrict__ out, long ldo) {
+  using S = RowsSmem<G, NP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *xs = smem + S::x_at, *raw = smem + S::raw_at;
+  float* scale = reinterpret_cast<float*>(smem + S::scale_at);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::bar_at);
+  uint64_t *raw_full = bars, *raw_empty = raw_full + kRawStages, *x_full = raw_empty + kRawStages,
+           *x_empty = x_full + kXStages, *dec_full = x_empty + kXStages, *dec_empty = dec_full + S::kDecoded,
+           *sum_full = dec_empty + S::kDecoded, *sum_empty = sum_full + 8, *scale_full = sum_empty + 8,
+           *drain = scale_full + kScaleSlots;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + kIssuers);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_at + 1);
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = splits > 1 ? (int)cluster_rank() : 0, unit = blockIdx.x / splits;
+  const int k0 = kt_n * rank / splits, steps = kt_n * (rank + 1) / splits - k0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRawStages; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], 4);
+    for (int i = 0; i < kXStages; ++i) mbar_init(&x_full[i], 1), mbar_init(&x_empty[i], 4 * kTotals);
+    for (int i = 0; i < S::kDecoded; ++i) mbar_init(&dec_full[i], 4), mbar_init(&dec_empty[i], 4 * kTotals);
+    for (int i = 0; i < 8; ++i) mbar_init(&sum_full[i], 1), mbar_init(&sum_empty[i], 4 * kTotals);
+    for (int i = 0; i < kScaleSlots; ++i) mbar_init(&scale_full[i], 4);
+    for (int i = 0; i < kIssuers; ++i) mbar_init(&drain[i], 1);
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_at, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();
+  const uint32_t tmem = *tmem_at;
+  // A wait that gives up raises `abort`, and every role ends; the outputs are then written as NaN.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_wait(bar, parity, abort, kWaitBudgetNs)) return true;
+    *abort = 1;
+    return false;
+  };
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
+
+  constexpr int kMine = NP / kTotals;  // tokens of a totals warp
+  const bool totals = warp >= kFirstTotals && warp < kFirstDecoder;
+  const int t_first = totals ? (warp - kFirstTotals) / 4 * kMine : 0;
+  uint64_t acc[kMine / 2];  // totals of row 32 q + lane, two tokens each
+#pragma unroll
+  for (int i = 0; i < kMine / 2; ++i) acc[i] = 0;
+
+  if (warp == 0 || warp == 3) {  // copies of the matrix; of x
+    pdl_wait();
+    fence_proxy_async_global();
+    const uint64_t policy = l2_policy_evict_first();
+    // One after the other through `stages` places.
+    auto copies = [&](auto stages, uint64_t* full, uint64_t* empty, auto copy) {
+      constexpr int n = decltype(stages)::value;
+      int at = 0, issued = 0;
+      uint32_t phase = 0;
+      for (; issued < steps; ++issued) {
+        if (!wait_warp(&empty[at], phase ^ 1)) break;
+        if (elect_one()) copy(&full[at], at, k0 + issued);
+        __syncwarp();
+        if (++at == n) at = 0, phase ^= 1;
+      }
+      // no copy may be under way when the CTA ends
+      for (int i = issued > n ? issued - n : 0; i < issued; ++i) mbar_wait_drain(&full[i % n], i / n & 1, kWaitBudgetNs);
+    };
+    if (warp == 0) {
+      copies(std::integral_constant<int, kRawStages>(), raw_full, raw_empty, [&](uint64_t* bar, int at, int k) {
+        mbar_arrive_expect_tx(bar, S::kRawTx);
+        load_4d(raw + at * S::kRaw, &map_w, bar, k, unit * 8, policy);
+      });
+    } else {
+      copies(std::integral_constant<int, kXStages>(), x_full, x_empty, [&](uint64_t* bar, int at, int k) {
+        mbar_arrive_expect_tx(bar, S::kX);
+        tma_load_2d_nohint(xs + at * S::kX, &map_x, bar, k * kTileK, 0);
+        tma_load_2d_nohint(xs + at * S::kX + S::kX / 2, &map_x, bar, k * kTileK + 64, 0);
+      });
+    }
+    __syncwarp();
+  } else if (warp <= kIssuers) {
+    constexpr uint32_t idesc = umma_idesc(sizeof(typename A::Raw) == 2 && A::kMagic == Bf16::kMagic ? 1u : 0u, kM, NP);
+    bool any = false;
+    for (int batch = warp - 1; batch < steps * S::kBatches; batch += kIssuers) {
+      const int i = batch / S::kBatches, g0 = batch % S::kBatches * S::kBatch;  // K position, first group
+      const int xi = i % kXStages, di = i % S::kDecoded, bi = batch % S::kPlaces;
+      if (!wait_warp(&x_full[xi], i / kXStages & 1) || !wait_warp(&dec_full[di], i / S::kDecoded & 1) ||
+          !wait_warp(&sum_empty[bi], (batch / S::kPlaces & 1) ^ 1))
+        break;
+      tc_fence_after();
+      any = true;
+      if (elect_one()) {
+        const uint64_t b0 = umma_desc_sw128(smem_u32(xs + xi * S::kX));
+        const uint32_t a0 = tmem + S::kDecodedAt + di * 64, d0 = tmem + bi * S::kBatch * S::kSumCols;
+#pragma unroll
+        for (int gr = 0; gr < S::kBatch; ++gr)
+#pragma unroll
+          for (int k = 0; k < G / 16; ++k) {
+            const int at = (g0 + gr) * G + 16 * k;  // column; x has 64 of them per swizzled half
+            mma_f16_tmem_a(d0 + gr * S::kSumCols, a0 + at / 2, b0 + (at / 64 * (S::kX / 2 / 16) + at % 64 / 8), idesc,
+                           k ? 1u : 0u);
+          }
+        tc_commit(&sum_full[bi]);
+      }
+      __syncwarp();
+    }
+    if (any) {
+      if (elect_one()) tc_commit(&drain[warp - 1]);
+      __syncwarp();
+      mbar_wait_drain(&drain[warp - 1], 0, kWaitBudgetNs);
+    }
+    __syncwarp();
+  } else if (totals) {
+    const int q = warp & 3, row = 32 * q + lane;
+    const uint32_t from = tmem + ((uint32_t)(32 * q) << 16) + t_first;
+    bool ok = true;
+    for (int i = 0; i < steps && ok; ++i) {
+      const int ci = i % kScaleSlots;
+      ok = wait(&scale_full[ci], i / kScaleSlots & 1);
+#pragma unroll
+      for (int g0 = 0; g0 < S::kGroups; g0 += S::kBatch) {
+        const int batch = i * S::kBatches + g0 / S::kBatch, bi = batch % S::kPlaces;
+        ok = ok && wait(&sum_full[bi], batch / S::kPlaces & 1);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (g0 + S::kBatch == S::kGroups && lane == 0) {  // these products, and with them all of the K position's, are done
+          mbar_arrive(&dec_empty[i % S::kDecoded]);
+          mbar_arrive(&x_empty[i % kXStages]);
+        }
+#pragma unroll
+        for (int gr = g0; gr < g0 + S::kBatch; ++gr) {
+          const float s = scale[(ci * S::kGroups + gr) * kM + row];
+          const uint64_t s2 = f32x2_pack(s, s);
+          uint64_t v[kMine / 2];
+          const uint32_t at = from + (bi * S::kBatch + gr - g0) * S::kSumCols;
+          if constexpr (kMine == 8) {
+            tmem_ld8_pairs(at, v);
+          } else {
+#pragma unroll
+            for (int n = 0; n < kMine; n += 16) tmem_ld16_pairs(at + n, *reinterpret_cast<uint64_t(*)[8]>(v + n / 2));
+          }
+          tmem_wait_ld();
+#pragma unroll
+          for (int n = 0; n < kMine / 2; ++n) f32x2_fma(acc[n], v[n], s2);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sum_empty[bi]);
+      }
+    }
+  } else {
+    // row 32 q + lane of the group's K positions
+    const int q = warp & 3, row = 32 * q + lane, tile = row / kTileN, h = row / 8 % 2, g = row % 8;
+    const uint32_t magic = magic_register<A>();
+    for (int i = (warp - kFirstDecoder) / 4; i < steps; i += kDecoders) {
+      const int ri = i % kRawStages, di = i % S::kDecoded, ci = i % kScaleSlots;
+      const bool ok = wait(&raw_full[ri], i / kRawStages & 1) && wait(&dec_empty[di], (i / S::kDecoded & 1) ^ 1);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const uint8_t* from = raw + ri * S::kRaw + tile * S::kTile;
+      // Pieces t of the row's 64 bytes.  Each pair of rows begins at another one, so that eight rows read all of the banks;
+      // the pieces are then put in their order.
+      uint4 w[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint4*>(from + row % 16 * 64 + ((t ^ (row >> 1 & 3)) << 4));
+      if (row & 2) swap(w[0], w[1]), swap(w[2], w[3]);
+      if (row & 4) swap(w[0], w[2]), swap(w[1], w[3]);
+#pragma unroll
+      for (int gr = 0; gr < S::kGroups; ++gr) {
+        const uint16_t b = *reinterpret_cast<const uint16_t*>(from + kTileQ + 32 * gr + 4 * g + 2 * h);
+        scale[(ci * S::kGroups + gr) * kM + row] = __uint_as_float((uint32_t)b << 16);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // words 2 half, 2 half + 1 of each piece: columns 64 half .. + 63
+        uint32_t p[32];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          uint32_t v[4];
+          decode_word<A>(half ? w[t].z : w[t].x, magic, v);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) p[4 * t + k] = v[k];
+          decode_word<A>(half ? w[t].w : w[t].y, magic, v);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) p[16 + 4 * t + k] = v[k];
+        }
+        tmem_st32(tmem + S::kDecodedAt + di * 64 + 32 * half + ((uint32_t)(32 * q) << 16), p);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&raw_empty[ri]);
+        mbar_arrive(&scale_full[ci]);
+        mbar_arrive(&dec_full[di]);
+      }
+    }
+  }
+  __syncwarp();
+  const float bad = __uint_as_float(0x7FC00000u);
+  const int row = 32 * (warp & 3) + lane, n = unit * kM + row;
+  // x and the tiles have been used: with more splits than one their place takes the totals, [token][row]
+  float* part = reinterpret_cast<float*>(smem);
+  if (splits > 1) __syncthreads();
+  if (totals) {
+    const bool failed = *abort;
+#pragma unroll
+    for (int t = 0; t < kMine; ++t) {
+      float v[2];
+      f32x2_unpack(acc[t / 2], v[0], v[1]);
+      const int token = t_first + t;
+      const float total = failed ? bad : v[t % 2];
+      if (token >= T) continue;
+      if (splits > 1)
+        part[token * kM + row] = total;
+      else if (n < N)
+        out[(size_t)token * ldo + n] = A::of(total);
+    }
+  }
+  if (splits > 1) {
+    __syncthreads();
+    cluster_sync();
+    for (int i = rank * kRowsThreads + threadIdx.x; i < T * kM; i += splits * kRowsThreads) {
+      float sum = 0.0f;
+      for (int k = 0; k < splits; ++k) sum += load_cluster(smem_u32(part + i), k);
+      const int m = unit * kM + i % kM;
+      if (m < N) out[(size_t)(i / kM) * ldo + m] = A::of(sum);
+    }
+    cluster_sync();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename A, int G, int NP>
+cudaError_t run_rows(const void* x, long ldx, int T, const void* packed, int N, int K, void* out, long ldo,
+                     cudaStream_t stream) {
+  using S = RowsSmem<G, NP>;
+  static DeviceFlags smem_set;
+  cudaError_t e = set_max_dynamic_smem(rows_kernel<A, G, NP>, S::total, smem_set);
+  if (e != cudaSuccess) return e;
+  const int kt = K / kTileK, units = (N - 1) / kM + 1, sms = num_sms_of_current_device();
+  int splits = 1;
+  while (splits < 8 && units * splits * 2 <= sms && kt >= 8 * splits) splits *= 2;
+  CUtensorMap map_w, map_x;
+  const uint64_t tb = S::kTile, row_tiles = (N - 1) / kTileN + 1;
+  const uint64_t dims[4] = {tb / 8, 1, (uint64_t)kt, row_tiles}, strides[3] = {tb, tb, kt * tb};
+  const uint32_t box[4] = {S::kTile / 8, 1, 1, 8};
+  if (encode_4d_words(&map_w, packed, dims, strides, box) != FBMOE_OK ||
+      encode_strided_2d(&map_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, K, T, (uint64_t)ldx * 2, 64, NP,
+                        CU_TENSOR_MAP_SWIZZLE_128B) != FBMOE_OK)
+    return cudaErrorUnknown;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(units * splits);
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = S::total;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, rows_kernel<A, G, NP>, map_w, map_x, T, N, kt, splits,
+                            reinterpret_cast<typename A::Raw*>(out), ldo);
+}
+
+// Which kernel, by how much there is to spread over the SMs.  tiles_kernel reads the matrix once per 16 tokens and starts and
+// ends at once; rows_kernel reads it once, and costs 4 us before its first and after its last product.  Measured, tiles /
+// rows, in us (G = 128; 32 moves the same way):
+//   N x K          tiles to read    T = 8          T = 16         T = 64
+//   1024 x 4096    2048             3.2 / 5.6      4.0 / 5.7      6.1 / 7.3
+//   7168 x 2048    7168             4.6 / 7.4      7.0 / 7.8      18.0 / 10.2
+//   4096 x 7168    14336            10.7 / 10.0    11.4 / 10.4    32.3 / 12.7
+//   18432 x 7168   64512            24.4 / 23.6    31.8 / 23.6    98.6 / 28.3
+//   256 x 14336    1792             8.0 / 8.5      9.9 / 8.8      16.1 / 11.1
+// So rows_kernel takes more than 8 tokens if tiles_kernel would read more than 8192 tiles, or if K is so long that each of
+// its warps has twelve or more in a row.
+bool rows_pay(int T, int N, int K) {
+  const long kt = K / kTileK, tiles = ((long)(N - 1) / kTileN + 1) * kt * ((T + 15) / 16);
+  return T > 8 && (tiles > 8192 || kt >= 12 * kWarps);
+}
+
 template <typename A, int G>
 cudaError_t run_linear(const void* x, long ldx, int T, const void* packed, int N, int K, void* out, long ldo,
                        cudaStream_t stream) {
@@ -64,9 +458,14 @@ cudaError_t run_linear(const void* x, long ldx, int T, const void* packed, int N
   const Raw* xp = reinterpret_cast<const Raw*>(x);
   const uint8_t* wp = reinterpret_cast<const uint8_t*>(packed);
   Raw* op = reinterpret_cast<Raw*>(out);
+  if (rows_pay(T, N, K)) {
+    if (T <= 16) return run_rows<A, G, 16>(x, ldx, T, packed, N, K, out, ldo, stream);
+    if (T <= 32) return run_rows<A, G, 32>(x, ldx, T, packed, N, K, out, ldo, stream);
+    return run_rows<A, G, 64>(x, ldx, T, packed, N, K, out, ldo, stream);
+  }
   if (T <= 8)
-    return launch_pdl(linear_kernel<A, G, 1>, dim3(nt), dim3(kWarps * 32), 0, stream, xp, ldx, T, wp, N, K, op, ldo);
-  return launch_pdl(linear_kernel<A, G, 2>, dim3(nt, (unsigned)((T + 15) / 16)), dim3(kWarps * 32), 0, stream, xp, ldx,
+    return launch_pdl(tiles_kernel<A, G, 1>, dim3(nt), dim3(kWarps * 32), 0, stream, xp, ldx, T, wp, N, K, op, ldo);
+  return launch_pdl(tiles_kernel<A, G, 2>, dim3(nt, (unsigned)((T + 15) / 16)), dim3(kWarps * 32), 0, stream, xp, ldx,
                     T, wp, N, K, op, ldo);
 }
 template <typename A>

@@ -211,6 +211,97 @@ def test_linear_large_values(fbmoe_lib):
     check_linear(fbmoe_lib.linear_w4(x, p), x, v, 128)
 
 
+# More than 8 tokens with a K of 12288 or more, or with more than 8192 tiles to read: the kernel of 128 rows per CTA.
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("T,N,K", [(9, 1, 12288), (16, 17, 12416), (17, 130, 12288), (33, 257, 12544), (64, 640, 14336),
+                                   (64, 33000, 128), (16, 18500, 1024), (20, 9000, 1152), (31, 2100, 4096)])
+def test_linear_rows(fbmoe_lib, dtype, G, T, N, K):
+    p, v = random_packed(N, K, G, T + N)
+    x = torch.randn((T, K), generator=torch.Generator().manual_seed(K)).to(dtype).cuda()
+    y = fbmoe_lib.linear_w4(x, p, N)
+    check_linear(y, x, v, G)
+    for _ in range(3):
+        assert torch.equal(y, fbmoe_lib.linear_w4(x, p, N))
+
+
+def test_linear_rows_every_token_count(fbmoe_lib):
+    p, v = random_packed(130, 12288, 128, 5)
+    x = torch.randn((64, 12288), generator=torch.Generator().manual_seed(1)).to(BF16).cuda()
+    for T in range(7, 65):
+        y = fbmoe_lib.linear_w4(x[:T], p, 130)
+        assert tuple(y.shape) == (T, 130)
+        check_linear(y, x[:T], v, 128)
+
+
+@pytest.mark.parametrize("T,N,K", [(16, 8192, 2048), (16, 8193, 2048), (64, 2049, 2048), (64, 2048, 2048), (64, 16, 12160),
+                                   (64, 16, 12288), (8, 16, 12288)])
+def test_linear_on_both_sides_of_the_choice(fbmoe_lib, T, N, K):
+    p, v = random_packed(N, K, 64, T + N)
+    x = torch.randn((T, K), generator=torch.Generator().manual_seed(K)).to(BF16).cuda()
+    check_linear(fbmoe_lib.linear_w4(x, p, N), x, v, 64)
+
+
+def test_linear_rows_strides_and_bad_values(fbmoe_lib):
+    """Rows of a wider tensor in, columns of a wider tensor out; a NaN or an infinity spoils its token's outputs only, a NaN
+    scale its row's."""
+    N, K = 150, 12288
+    p, v = random_packed(N, K, 64, 9)
+    for T in (9, 20, 64):
+        big = torch.randn((T + 3, K + 16), generator=torch.Generator().manual_seed(T)).to(F16).cuda()
+        big[T:], big[:, :8], big[:, -8:] = float("nan"), float("nan"), float("nan")  # what is not x
+        x = big[:T, 8:-8]
+        out = torch.full((T + 1, N + 11), 7.0, dtype=F16, device="cuda")
+        y = fbmoe_lib.linear_w4(x, p, N, out=out[:T, 5:N + 5])
+        check_linear(y, x, v, 64)
+        assert (out[:, :5] == 7).all() and (out[:, N + 5:] == 7).all() and (out[T] == 7).all()
+        bad = x.clone()
+        bad[1, 7], bad[2, 12000] = float("nan"), float("inf")
+        z = fbmoe_lib.linear_w4(bad, p, N)
+        assert z[1].isnan().all() and not z[2].isfinite().any()
+        keep = [t for t in range(T) if t not in (1, 2)]
+        assert torch.equal(z[keep], y[keep])
+    q = p.clone()
+    q[0, 50, 1024:1026] = torch.tensor([0xC0, 0x7F], dtype=torch.uint8)  # row 0's scale in K position 50: NaN
+    z = fbmoe_lib.linear_w4(x, q, N)
+    assert z[:, 0].isnan().all() and torch.equal(z[:, 1:], y[:, 1:])
+
+
+def test_linear_rows_on_two_streams(fbmoe_lib):
+    """Clusters and single CTAs that take all of an SM's tensor memory, of two calls at once."""
+    calls = []
+    for T, N, K in ((64, 300, 12288), (33, 4096, 4096), (12, 19000, 1024)):
+        p, _ = random_packed(N, K, 64, N)
+        x = torch.randn((T, K), generator=torch.Generator().manual_seed(T)).to(BF16).cuda()
+        calls.append((x, p, N, fbmoe_lib.linear_w4(x, p, N)))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    results = []
+    for i in range(30):
+        for j, s in enumerate(streams):
+            x, p, N, ref = calls[(i + j) % 3]
+            with torch.cuda.stream(s):
+                results.append((fbmoe_lib.linear_w4(x, p, N), ref))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, ref) for y, ref in results)
+
+
+def test_linear_rows_captured(fbmoe_lib):
+    """Two layers, one reading the other's result, captured once and replayed over new inputs."""
+    p1, _ = random_packed(12288, 1024, 128, 1)
+    p2, _ = random_packed(512, 12288, 32, 2)
+    x = torch.zeros((32, 1024), dtype=BF16, device="cuda")
+    inputs = [torch.randn((32, 1024), generator=torch.Generator().manual_seed(i)).to(BF16).cuda() for i in range(3)]
+    eager = [fbmoe_lib.linear_w4(fbmoe_lib.linear_w4(i, p1), p2) for i in inputs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fbmoe_lib.linear_w4(fbmoe_lib.linear_w4(x, p1), p2)
+    for i, e in zip(inputs * 2, eager * 2):
+        x.copy_(i)
+        graph.replay()
+        assert torch.equal(y, e)
+
+
 # ------------------------------------------------------------------ the MoE layer
 class Case:
     def __init__(self, lib, T, E, offset, H, I, G1, G2, dtype, config, seed):
