@@ -69,9 +69,9 @@ int num_sms_of_current_device();
 // 2-D map of rows `row_bytes` apart; FBMOE_OK or FBMOE_ERR_DRIVER.
 int encode_strided_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t rows,
                       uint64_t row_bytes, uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle);
-// 4-D map of 8-byte elements without swizzle; strides in bytes.  FBMOE_OK or FBMOE_ERR_DRIVER.
+// 4-D map of 8-byte elements; strides in bytes.  FBMOE_OK or FBMOE_ERR_DRIVER.
 int encode_4d_words(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
-                    const uint32_t (&box)[4]);
+                    const uint32_t (&box)[4], CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_NONE);
 
 // Offsets (bytes) of the sub-buffers inside the caller-provided workspace.
 struct Layout {

@@ -127,12 +127,12 @@ int encode_strided_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* b
 }
 
 int encode_4d_words(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
-                    const uint32_t (&box)[4]) {
+                    const uint32_t (&box)[4], CUtensorMapSwizzle swizzle) {
   if (!get_encode()) return FBMOE_ERR_DRIVER;
   const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, st[3] = {strides[0], strides[1], strides[2]};
   const cuuint32_t b[4] = {box[0], box[1], box[2], box[3]}, estr[4] = {1, 1, 1, 1};
   const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_INT64, 4, const_cast<void*>(base), d, st, b, estr,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? FBMOE_OK : FBMOE_ERR_DRIVER;
 }

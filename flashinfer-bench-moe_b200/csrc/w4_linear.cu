@@ -5,19 +5,22 @@
 // the tiles along K in turn and their partial sums are added in warp order through shared memory.  Bound by latency.
 //
 // rows_kernel: 128 rows of the matrix are the M of a tcgen05 product, up to 64 tokens its N.  Per K position (128 columns)
-// one tensor copy brings the eight row tiles and two bring x; four warps decode, a thread per row, to exact 16-bit floats q
+// two tensor copies bring the eight row tiles' values and scales and two bring x; four warps decode, a thread per row, to
+// exact 16-bit floats q
 // in tensor memory, the product's A operand; the tensor core sums each scale group into columns of its own (x and q exact,
 // sums fp32), and eight warps, a thread per row and half of the tokens, add s times that sum to totals in registers.  So no
 // weight is rounded and the matrix is read once for all tokens.  A cluster of S CTAs splits K where there are fewer blocks
 // of rows than half the SMs; their totals are added in rank order through shared memory.
 //
-// N = 18432, K = 7168, G = 128 on a B200: 23.6 us for 9 to 16 tokens, 24.7 for 32, 28.3 for 64 (reading alone 10.5 to 10.9),
-// tiles_kernel 30 to 99; G = 32: 27.5, 30.4, 45.8.  What it cost on the way, at 64 tokens: 50 us with the decoded tile in
+// N = 18432, K = 7168, G = 128 on a B200: 22.5 us for 9 to 16 tokens, 24.1 for 32, 27.6 for 64 (reading alone 10.5 to 10.9),
+// tiles_kernel 30 to 99; G = 32: 26.1, 29.1, 41.9.  What it cost on the way, at 64 tokens: 50 us with the decoded tile in
 // shared memory (32 KB written and 32 KB read per position: 1350 cycles), 44 with it in tensor memory, 32.5 with two issuing
 // threads, one commit per position and two groups of decoders, 31.2 with lanes chosen by elect.sync, 28.4 with two groups of
-// totals (in turns by position in place of by tokens: 32.9).  Bound by the roles' waits on one another: a position takes 0.33 to
-// 0.42 us, and without the decoding it would take 20.3 us for one token (29.1 for 64, before the second group of totals),
-// without most of the products 23.4 (30.3), without the totals' sums 22.4 (25.2); four groups of decoders are no faster.
+// totals (in turns by position in place of by tokens: 32.9), 27.3 with the values swizzled by the copy in place of exchanged
+// in registers.  Bound by instructions (60 to 64% of the issue slots, the decoding above all) and by the roles' waits on one
+// another, 0.35 to 0.43 us a position.  Before that last step, without the decoding's arithmetic 21.6 us at 16 tokens and 25.8
+// at 64, without the totals' sums 23.1 and 25.2, without either, the stores and most products 16.8 and 17.9, of which the
+// reading is less than 1.  More places, four groups of decoders or two CTAs per SM are no faster.
 #include <type_traits>
 #include "fbmoe.h"
 #include "fbmoe_launch.h"
@@ -87,7 +90,8 @@ constexpr uint64_t kWaitBudgetNs = 4000000000ull;
 
 template <int G, int NP>
 struct RowsSmem {
-  static constexpr int kTile = tile_bytes(G), kRawTx = 8 * kTile, kRaw = (kRawTx + 127) / 128 * 128;
+  static constexpr int kTile = tile_bytes(G), kScaleBytes = kTile - kTileQ, kRawTx = 8 * kTile;
+  static constexpr int kRaw = 9 * 1024;  // values, then scales
   static constexpr int kX = NP * kTileK * 2;
   static constexpr int kGroups = kTileK / G;
   // Tensor memory: the first half holds group sums, the other decoded tiles of 64 columns (six of those were no faster).
@@ -109,11 +113,6 @@ struct RowsSmem {
   static constexpr int total = used > 116 * 1024 ? used : 116 * 1024;
 };
 
-__device__ __forceinline__ void swap(uint4& a, uint4& b) {
-  const uint4 c = a;
-  a = b;
-  b = c;
-}
 // One lane of a warp that has not diverged.  The compiler then keeps what is the same in all lanes in uniform registers, as
 // copies and products take it; a branch on the lane's number made the whole 1 to 2 us slower.
 __device__ __forceinline__ bool elect_one() {
@@ -157,7 +156,7 @@ __device__ __forceinline__ void load_4d(void* dst, const CUtensorMap* map, uint6
 
 template <typename A, int G, int NP>
 __global__ void __launch_bounds__(kRowsThreads, 1)
-    rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, int T, int N, int kt_n,
+    rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_x, int T, int N, int kt_n,
                 int splits, typename A::Raw* __restrict__ out, long ldo) {
   using S = RowsSmem<G, NP>;
   extern __shared__ uint8_t smem_raw[];
@@ -230,6 +229,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       copies(std::integral_constant<int, kRawStages>(), raw_full, raw_empty, [&](uint64_t* bar, int at, int k) {
         mbar_arrive_expect_tx(bar, S::kRawTx);
         load_4d(raw + at * S::kRaw, &map_w, bar, k, unit * 8, policy);
+        load_4d(raw + at * S::kRaw + 8 * kTileQ, &map_s, bar, k, unit * 8, policy);
       });
     } else {
       copies(std::integral_constant<int, kXStages>(), x_full, x_empty, [&](uint64_t* bar, int at, int k) {
@@ -321,17 +321,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       const bool ok = wait(&raw_full[ri], i / kRawStages & 1) && wait(&dec_empty[di], (i / S::kDecoded & 1) ^ 1);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      const uint8_t* from = raw + ri * S::kRaw + tile * S::kTile;
-      // Pieces t of the row's 64 bytes.  Each pair of rows begins at another one, so that eight rows read all of the banks;
-      // the pieces are then put in their order.
-      uint4 w[4];
+      const uint8_t *from = raw + ri * S::kRaw, *sc = from + 8 * kTileQ + tile * S::kScaleBytes;
+      uint4 w[4];  // pieces t of the row's 64 bytes, swizzled by the row's bits 1 and 2
 #pragma unroll
-      for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint4*>(from + row % 16 * 64 + ((t ^ (row >> 1 & 3)) << 4));
-      if (row & 2) swap(w[0], w[1]), swap(w[2], w[3]);
-      if (row & 4) swap(w[0], w[2]), swap(w[1], w[3]);
+      for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint4*>(from + row * 64 + ((t ^ (row >> 1 & 3)) << 4));
 #pragma unroll
       for (int gr = 0; gr < S::kGroups; ++gr) {
-        const uint16_t b = *reinterpret_cast<const uint16_t*>(from + kTileQ + 32 * gr + 4 * g + 2 * h);
+        const uint16_t b = *reinterpret_cast<const uint16_t*>(sc + 32 * gr + 4 * g + 2 * h);
         scale[(ci * S::kGroups + gr) * kM + row] = __uint_as_float((uint32_t)b << 16);
       }
 #pragma unroll
@@ -409,11 +405,14 @@ cudaError_t run_rows(const void* x, long ldx, int T, const void* packed, int N, 
   const int kt = K / kTileK, units = (N - 1) / kM + 1, sms = num_sms_of_current_device();
   int splits = 1;
   while (splits < 8 && units * splits * 2 <= sms && kt >= 8 * splits) splits *= 2;
-  CUtensorMap map_w, map_x;
+  CUtensorMap map_w, map_s, map_x;
   const uint64_t tb = S::kTile, row_tiles = (N - 1) / kTileN + 1;
-  const uint64_t dims[4] = {tb / 8, 1, (uint64_t)kt, row_tiles}, strides[3] = {tb, tb, kt * tb};
-  const uint32_t box[4] = {S::kTile / 8, 1, 1, 8};
-  if (encode_4d_words(&map_w, packed, dims, strides, box) != FBMOE_OK ||
+  const uint64_t dims_q[4] = {8, kTileN, (uint64_t)kt, row_tiles}, strides[3] = {64, tb, kt * tb};
+  const uint64_t dims_s[4] = {(uint64_t)S::kScaleBytes / 8, 1, (uint64_t)kt, row_tiles};
+  const uint32_t box_q[4] = {8, kTileN, 1, 8}, box_s[4] = {S::kScaleBytes / 8, 1, 1, 8};
+  if (encode_4d_words(&map_w, packed, dims_q, strides, box_q, CU_TENSOR_MAP_SWIZZLE_64B) != FBMOE_OK ||
+      encode_4d_words(&map_s, reinterpret_cast<const uint8_t*>(packed) + kTileQ, dims_s, strides, box_s,
+                      CU_TENSOR_MAP_SWIZZLE_NONE) != FBMOE_OK ||
       encode_strided_2d(&map_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, K, T, (uint64_t)ldx * 2, 64, NP,
                         CU_TENSOR_MAP_SWIZZLE_128B) != FBMOE_OK)
     return cudaErrorUnknown;
@@ -430,7 +429,7 @@ cudaError_t run_rows(const void* x, long ldx, int T, const void* packed, int N, 
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = splits > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, rows_kernel<A, G, NP>, map_w, map_x, T, N, kt, splits,
+  return cudaLaunchKernelEx(&cfg, rows_kernel<A, G, NP>, map_w, map_s, map_x, T, N, kt, splits,
                             reinterpret_cast<typename A::Raw*>(out), ldo);
 }
 
@@ -438,11 +437,12 @@ cudaError_t run_rows(const void* x, long ldx, int T, const void* packed, int N, 
 // ends at once; rows_kernel reads it once, and costs 4 us before its first and after its last product.  Measured, tiles /
 // rows, in us (G = 128; 32 moves the same way):
 //   N x K          tiles to read    T = 8          T = 16         T = 64
-//   1024 x 4096    2048             3.2 / 5.6      4.0 / 5.7      6.1 / 7.3
-//   7168 x 2048    7168             4.6 / 7.4      7.0 / 7.8      18.0 / 10.2
-//   4096 x 7168    14336            10.7 / 10.0    11.4 / 10.4    32.3 / 12.7
-//   18432 x 7168   64512            24.4 / 23.6    31.8 / 23.6    98.6 / 28.3
-//   256 x 14336    1792             8.0 / 8.5      9.9 / 8.8      16.1 / 11.1
+//   1024 x 4096    2048             3.2 / 5.5      4.0 / 5.6      6.1 / 7.0
+//   7168 x 2048    7168             4.6 / 7.2      7.0 / 7.5      18.0 / 9.9
+//   4096 x 7168    14336            10.7 / 9.9     11.4 / 10.0    32.3 / 12.4
+//   18432 x 7168   64512            24.4 / 22.4    31.8 / 22.5    98.6 / 27.6
+//   32001 x 7168   112056           31.5 / 43.8    49.6 / 43.9    170.7 / 52.6
+//   256 x 14336    1792             8.0 / 8.4      9.9 / 8.5      16.1 / 10.7
 // So rows_kernel takes more than 8 tokens if tiles_kernel would read more than 8192 tiles, or if K is so long that each of
 // its warps has twelve or more in a row.
 bool rows_pay(int T, int N, int K) {

@@ -20,7 +20,8 @@
 // the rows, stream the unit's tiles through their rings (w4_stream.cuh) and on into the next unit's; two finisher warps
 // add their partial sums in a fixed order, apply SwiGLU or the routing weight, store and report.  A unit takes an SM 3 to
 // 6 us at H = 7168, so phases and the end of the call are balanced to that; with a unit per warp or group of warps
-// (measured) they were not: 207 us in place of TODO64 us at T = 64.  Every order of summation depends on the sizes alone.
+// (measured) they were not: 202 us in place of 165 at T = 64.  Every order of summation depends on the sizes and the
+// routing alone.
 #include "fbmoe.h"
 #include "fbmoe_launch.h"
 #include "moe_route.cuh"
@@ -373,7 +374,7 @@ template <int G, int NT, bool UP, typename S, typename Wait>
 __device__ __forceinline__ bool consume(const LayerArgs& a, Shared& s, S& st, const Unit& u, const Span& w, float* part,
                                         const Wait& free_part) {
   const int lane = threadIdx.x & 31, g = lane >> 2;
-  const uint32_t flip = flip_register(), two = two_register();
+  const uint32_t flip = flip_register();
   float acc[4][NT][2] = {};
   if (row_group(s, u, threadIdx.x / 32) < row_groups(a, u)) {
     Places<NT, !UP> at;
@@ -391,10 +392,10 @@ __device__ __forceinline__ bool consume(const LayerArgs& a, Shared& s, S& st, co
       if (left > 1) at.advance();  // the last one is read twice
       st.ring.wait(&s.abort);
       const uint32_t words = st.ring.got + 16 * lane, scales = st.ring.got + 4 * g;
-      tile_product<G, NT, !UP, 0>(words, scales, x, flip, two, acc[0], keep);
-      tile_product<G, NT, !UP, tile_bytes(G)>(words, scales, x, flip, two, acc[1], keep);
-      tile_product<G, NT, !UP, 2 * tile_bytes(G)>(words, scales, x, flip, two, acc[2], keep);
-      tile_product<G, NT, !UP, 3 * tile_bytes(G)>(words, scales, x, flip, two, acc[3], reload);
+      tile_product<G, NT, !UP, 0>(words, scales, x, flip, acc[0], keep);
+      tile_product<G, NT, !UP, tile_bytes(G)>(words, scales, x, flip, acc[1], keep);
+      tile_product<G, NT, !UP, 2 * tile_bytes(G)>(words, scales, x, flip, acc[2], keep);
+      tile_product<G, NT, !UP, 3 * tile_bytes(G)>(words, scales, x, flip, acc[3], reload);
       at.load_scales(x);
       st.ring.release();
       st.fill(a, s);
@@ -754,10 +755,7 @@ cudaError_t run_moe(const MoeArgs& m) {
                              reinterpret_cast<int32_t*>(m.ws + L.topk_idx), reinterpret_cast<float*>(m.ws + L.topk_w), m.ws + L.xq,
                              reinterpret_cast<float*>(m.ws + L.xs), reinterpret_cast<Counters*>(m.ws + L.counters));
   if (e != cudaSuccess) return e;
-  int dev = 0, sms = 0;
-  e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return e;
+  const int sms = num_sms_of_current_device();
   if (m.group1 == 32) return pick_layer<A, 32>(m, L, sms);
   if (m.group1 == 64) return pick_layer<A, 64>(m, L, sms);
   return pick_layer<A, 128>(m, L, sms);

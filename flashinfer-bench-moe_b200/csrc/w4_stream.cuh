@@ -4,16 +4,15 @@
 //
 // Bytes in flight.  At 6.5 TB/s one SM takes 44 GB/s, and 1 to 2 us of latency under load ask for about 100 KB under way
 // per SM.  A ring belongs to one warp, which fills it itself: no producer warp, no empty barrier (a warp-wide sync orders
-// a slot's last read before its next copy).  A step is four tiles, contiguous along K, in two or four bulk copies of 1 to
-// 2 KB.  More under way is slower (plain streaming of 1056-byte copies on a B200: 6.8 TB/s with 100 KB per SM, 6.5 with
+// a slot's last read before its next copy).  A step is four tiles in one tensor copy.  More under way is slower (plain streaming of 1056-byte copies on a B200: 6.8 TB/s with 100 KB per SM, 6.5 with
 // 134, 5.6 with 200).
 //
 // Instructions.  86 cycles per two tiles and SM at that rate are 344 issue slots; the logic pipe takes two instructions a
 // cycle.  Decoding to pairs of 16-bit floats takes 7 logic instructions and 4 subtractions per word of eight weights, 242
 // instructions per two tiles in all: 84 to 90 cycles (measured, 16 warps, weights in shared memory), so the decoding
-// would be the limit.  As 8-bit integers a word takes 4: rotate, and (w & 0xF0F0F0F0) ^ 0x80808080 gives four bytes
-// 16 q in two's complement, twice.  The activations are two 8-bit planes of a 16-bit integer, x = s (256 hi + lo), in two
-// columns of one product; their sums are exact in 32 bits, which leaves half the slots free.
+// would be the limit.  As 8-bit integers a word takes 4: (w & 0xF0F0F0F0) ^ 0x80808080 of the word rotated to either side
+// gives four bytes 16 q in two's complement.  The activations are two 8-bit planes of a 16-bit integer, x = s (256 hi + lo),
+// in two columns of one product; their sums are exact in 32 bits, which leaves half the slots free.
 //
 // Activations: s is a power of two per token and 128 columns (32 for the layer's intermediate), so that the largest
 // |x / s| lies in [2^14, 2^15): a bf16 value within 2^-7 of the largest, an f16 value within 2^-4, is exact, a smaller
@@ -164,17 +163,6 @@ __device__ __forceinline__ uint32_t and_xor(uint32_t v, uint32_t flip) {
   asm("lop3.b32 %0, %1, 0xF0F0F0F0, %2, 0x6A;" : "=r"(r) : "r"(v), "r"(flip));
   return r;
 }
-// 2 v as a product: the shift would go to the logic pipe, which is the fuller one.
-__device__ __forceinline__ uint32_t twice(uint32_t v, uint32_t two) {
-  uint32_t r;
-  asm("mul.lo.u32 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(two));
-  return r;
-}
-__device__ __forceinline__ uint32_t two_register() {
-  uint32_t r;
-  asm volatile("mov.b32 %0, 2;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ uint32_t flip_register() {
   uint32_t r;
   asm volatile("mov.b32 %0, 0x80808080;" : "=r"(r));
@@ -202,7 +190,7 @@ struct Columns {
 // scales = slot + 4 * g) times the columns.  reload(j) is called once the columns' words 2j, 2j + 1 have been used.
 template <int G, int NT, bool FINE, int AT, typename Reload>
 __device__ __forceinline__ void tile_product(uint32_t words, uint32_t scales, const Columns<NT, FINE>& x, uint32_t flip,
-                                             uint32_t two, float (&acc)[NT][2], const Reload& reload) {
+                                             float (&acc)[NT][2], const Reload& reload) {
   const uint4 lo = lds128<AT>(words), hi = lds128<AT + 512>(words);
   const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
   uint32_t sw[4];

@@ -540,8 +540,8 @@ def dequantize_w4(packed: torch.Tensor, n: int = None, dtype: torch.dtype = torc
 
 def linear_w4(x: torch.Tensor, weight: torch.Tensor, n: int = None, out: torch.Tensor = None) -> torch.Tensor:
     """``x @ W^T`` for at most 64 tokens: x [T, K] bfloat16 or float16 (rows may be strided by a multiple of 8
-    elements), ``weight`` one packed [n, K] matrix; returns [T, n] in x's type, summed in fp32.  More tokens: a GEMM
-    on ``dequantize_w4(weight, n)``."""
+    elements), ``weight`` one packed [n, K] matrix; returns [T, n] in x's type, summed in fp32; ``out`` must not
+    overlap x.  More tokens: a GEMM on ``dequantize_w4(weight, n)``."""
     n, K, group = _w4_shape(weight, "weight", n)
     _require(weight.dim() == 3, "weight must be one packed matrix [ceil(N / 16), K / 128, tile]")
     _require(isinstance(x, torch.Tensor) and x.dtype in _W4_X_TYPES, "x must be bfloat16 or float16")

@@ -74,6 +74,6 @@ def fused_moe_w4(
         hidden_states,
         gemm1_weights,
         gemm2_weights,
-        local_expert_offset,
-        routed_scaling_factor,
+        int(local_expert_offset),
+        float(routed_scaling_factor),
     )

@@ -329,7 +329,8 @@ FBMOE_API int fbmoe_dequantize_w4(const void* packed, int64_t batch, int N, int 
 
 /* out[t, n] = sum over k of x[t, k] * w[n, k] for 0 <= T <= 64 tokens: x and out of
  * `type` (FBMOE_BF16 or FBMOE_F16), rows x_stride and out_stride elements apart
- * (x 16-byte aligned, x_stride a multiple of 8), sums in fp32. */
+ * (x 16-byte aligned, x_stride a multiple of 8; out overlaps neither x nor packed),
+ * sums in fp32.  A bounded wait that expires makes outputs NaN. */
 FBMOE_API int fbmoe_linear_w4(const void* x, int64_t x_stride, int type, int T, const void* packed, int N, int K,
                               int group, void* out, int64_t out_stride, void* stream);
 
