@@ -6,11 +6,10 @@
 //
 // rows_kernel: 128 rows of the matrix are the M of a tcgen05 product, up to 64 tokens its N.  Per K position (128 columns)
 // two tensor copies bring the eight row tiles' values and scales and two bring x; four warps decode, a thread per row, to
-// exact 16-bit floats q
-// in tensor memory, the product's A operand; the tensor core sums each scale group into columns of its own (x and q exact,
-// sums fp32), and eight warps, a thread per row and half of the tokens, add s times that sum to totals in registers.  So no
-// weight is rounded and the matrix is read once for all tokens.  A cluster of S CTAs splits K where there are fewer blocks
-// of rows than half the SMs; their totals are added in rank order through shared memory.
+// exact 16-bit floats q in tensor memory, the product's A operand; the tensor core sums each scale group into columns of its
+// own (x and q exact, sums fp32), and eight warps, a thread per row and half of the tokens, add s times that sum to totals in
+// registers.  So no weight is rounded and the matrix is read once for all tokens.  A cluster of S CTAs splits K where there
+// are fewer blocks of rows than half the SMs; their totals are added in rank order through shared memory.
 //
 // N = 18432, K = 7168, G = 128 on a B200: 22.5 us for 9 to 16 tokens, 24.1 for 32, 27.6 for 64 (reading alone 10.5 to 10.9),
 // tiles_kernel 30 to 99; G = 32: 26.1, 29.1, 41.9.  What it cost on the way, at 64 tokens: 50 us with the decoded tile in
@@ -156,7 +155,8 @@ __device__ __forceinline__ void load_4d(void* dst, const CUtensorMap* map, uint6
 
 template <typename A, int G, int NP>
 __global__ void __launch_bounds__(kRowsThreads, 1)
-    rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_x, int T, int N, int kt_n,
+    rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
+                const __grid_constant__ CUtensorMap map_x, int T, int N, int kt_n,
                 int splits, typename A::Raw* __restrict__ out, long ldo) {
   using S = RowsSmem<G, NP>;
   extern __shared__ uint8_t smem_raw[];

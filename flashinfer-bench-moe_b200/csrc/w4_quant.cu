@@ -5,10 +5,13 @@
 // fp32 quotient, 0 where s is not positive.  A group that holds a NaN or an infinity gets the scale NaN.
 // Reader: v = q * s, exact in fp32 (4 bits times 8), rounded once to the output type.
 //
-// Both are bound by HBM.  One warp per tile: lane l = 4g + t owns rows g and g + 8, columns 32j + 8t .. + 7, which are
-// its packed words, so values go from the loads to the packed stores without shared memory: a quad reads 32
-// contiguous columns of a row, a half tile is stored as one coalesced 512-byte row of 16-byte words, and a group's
-// maximum is at most two shuffles over the quad.
+// The reader is bound by HBM (4096 x 7168 to bf16: 12.2 us, 6.0 TB/s; 8 x 7168 x 2048, G = 32, to fp32: 5.6 TB/s), the
+// quantiser by its arithmetic: about 16 instructions per weight and lane, 60 to 72% of the issue slots (4096 x 7168 bf16: 20
+// us, of which reading and writing alone would take 11).  One warp per tile: lane l = 4g + t owns rows g and g + 8, columns
+// 32j + 8t .. + 7, which are its packed words, so values go from the loads to the packed stores without shared memory: a
+// quad reads 32 contiguous columns of a row, a half tile is stored as one coalesced 512-byte row of 16-byte words, and a
+// group's maximum is at most two shuffles over the quad.
+#include <limits.h>
 #include "fbmoe.h"
 #include "fbmoe_launch.h"
 #include "w4_common.cuh"
@@ -144,7 +147,7 @@ __device__ __forceinline__ uint32_t scale_bits(float m) {
 constexpr uint32_t kZeroWord = 0x44444444u;  // rotl32(0x88888888, 3): q = 0
 
 template <int TYPE, int G, bool GIVEN>
-__global__ void __launch_bounds__(kWarps * 32, TYPE == kF32 ? 2 : 3) quantize_kernel(const void* __restrict__ w,
+__global__ void __launch_bounds__(kWarps * 32, TYPE == kF32 ? 2 : 4) quantize_kernel(const void* __restrict__ w,
                                                                const float* __restrict__ block_scale,
                                                                const uint16_t* __restrict__ given, uint32_t tiles, int N,
                                                                int K, uint8_t* __restrict__ packed) {
@@ -153,58 +156,58 @@ __global__ void __launch_bounds__(kWarps * 32, TYPE == kF32 ? 2 : 3) quantize_ke
   const uint32_t kt_n = K / kTileK, nt_n = (N + kTileN - 1) / kTileN;
   pdl_wait();
   pdl_trigger();
-  for (uint32_t tile = blockIdx.x * kWarps + (threadIdx.x >> 5); tile < tiles; tile += gridDim.x * kWarps) {
-    const uint32_t row_tile = tile / kt_n, kt = tile - row_tile * kt_n, b = row_tile / nt_n, nt = row_tile - b * nt_n;
-    uint8_t* out = packed + (size_t)tile * tile_bytes(G);
-    uint32_t scale_word[kGroups] = {};
-    Raw8<TYPE> raw[2][4];
+  const uint32_t tile = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (tile >= tiles) return;
+  const uint32_t row_tile = tile / kt_n, kt = tile - row_tile * kt_n, b = row_tile / nt_n, nt = row_tile - b * nt_n;
+  uint8_t* out = packed + (size_t)tile * tile_bytes(G);
+  uint32_t scale_word[kGroups] = {};
+  Raw8<TYPE> raw[2][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = nt * kTileN + 8 * h + g;
-      const size_t at = ((size_t)b * N + row) * K + (size_t)kt * kTileK + 8 * t;
+  for (int h = 0; h < 2; ++h) {
+    const int row = nt * kTileN + 8 * h + g;
+    const size_t at = ((size_t)b * N + row) * K + (size_t)kt * kTileK + 8 * t;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (row < N) raw[h][j].load(w, at + 32 * j);
-        else raw[h][j].zero();
-      }
+    for (int j = 0; j < 4; ++j) {
+      if (row < N) raw[h][j].load(w, at + 32 * j);
+      else raw[h][j].zero();
     }
-    // a tile lies inside one 128 x 128 block
-    const float bs = TYPE == kE4m3 ? __ldg(block_scale + ((size_t)b * ((N + 127) / 128) + nt / 8) * kt_n + kt) : 1.0f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = nt * kTileN + 8 * h + g;
-      uint32_t word[4];
-#pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) {
-        float v[kPer][8], m = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          raw[h][gr * kPer + j].widen(v[j], bs);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) m = max_abs_nan(m, v[j][i]);
-        }
-        m = max_abs_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max_abs_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        uint32_t sb;
-        if (GIVEN)
-          sb = row < N ? given[((size_t)b * N + row) * (K / G) + (size_t)kt * kGroups + gr] : 0u;
-        else
-          sb = scale_bits(m);
-        if (!(m <= 3.402823466e38f)) sb = 0x7FC0u;  // an infinity or a NaN among them
-        const float s = __uint_as_float(sb << 16);
-        float r;
-        asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
-        const bool use = s >= kMinNormal && s <= 3.402823466e38f;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) word[gr * kPer + j] = use ? quantize8<GIVEN>(v[j], s, r) : kZeroWord;
-        scale_word[gr] |= sb << (16 * h);
-      }
-      *reinterpret_cast<uint4*>(out + 512 * h + 16 * lane) = make_uint4(word[0], word[1], word[2], word[3]);
-    }
-#pragma unroll
-    for (int gr = 0; gr < kGroups; ++gr)
-      if (t == 0) *reinterpret_cast<uint32_t*>(out + kTileQ + 32 * gr + 4 * g) = scale_word[gr];
   }
+  // a tile lies inside one 128 x 128 block
+  const float bs = TYPE == kE4m3 ? __ldg(block_scale + ((size_t)b * ((N + 127) / 128) + nt / 8) * kt_n + kt) : 1.0f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = nt * kTileN + 8 * h + g;
+    uint32_t word[4];
+#pragma unroll
+    for (int gr = 0; gr < kGroups; ++gr) {
+      float v[kPer][8], m = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        raw[h][gr * kPer + j].widen(v[j], bs);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max_abs_nan(m, v[j][i]);
+      }
+      m = max_abs_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max_abs_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      uint32_t sb;
+      if (GIVEN)
+        sb = row < N ? given[((size_t)b * N + row) * (K / G) + (size_t)kt * kGroups + gr] : 0u;
+      else
+        sb = scale_bits(m);
+      if (!(m <= 3.402823466e38f)) sb = 0x7FC0u;  // an infinity or a NaN among them
+      const float s = __uint_as_float(sb << 16);
+      float r;
+      asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
+      const bool use = s >= kMinNormal && s <= 3.402823466e38f;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) word[gr * kPer + j] = use ? quantize8<GIVEN>(v[j], s, r) : kZeroWord;
+      scale_word[gr] |= sb << (16 * h);
+    }
+    *reinterpret_cast<uint4*>(out + 512 * h + 16 * lane) = make_uint4(word[0], word[1], word[2], word[3]);
+  }
+#pragma unroll
+  for (int gr = 0; gr < kGroups; ++gr)
+    if (t == 0) *reinterpret_cast<uint32_t*>(out + kTileQ + 32 * gr + 4 * g) = scale_word[gr];
 }
 
 // Eight consecutive values in the output type.
@@ -243,48 +246,50 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* 
   pdl_wait();
   pdl_trigger();
   for (uint32_t tile = blockIdx.x * kWarps + (threadIdx.x >> 5); tile < tiles; tile += gridDim.x * kWarps) {
-    const uint32_t row_tile = tile / kt_n, kt = tile - row_tile * kt_n, b = row_tile / nt_n, nt = row_tile - b * nt_n;
-    const uint8_t* in = packed + (size_t)tile * tile_bytes(G);
-    const uint4 q[2] = {__ldg(reinterpret_cast<const uint4*>(in + 16 * lane)),
-                        __ldg(reinterpret_cast<const uint4*>(in + 512 + 16 * lane))};
-    const uint32_t magic = magic_register<Bf16>();
-    uint32_t sw[128 / G];
+  const uint32_t row_tile = tile / kt_n, kt = tile - row_tile * kt_n, b = row_tile / nt_n, nt = row_tile - b * nt_n;
+  const uint8_t* in = packed + (size_t)tile * tile_bytes(G);
+  const uint4 q[2] = {__ldg(reinterpret_cast<const uint4*>(in + 16 * lane)),
+                      __ldg(reinterpret_cast<const uint4*>(in + 512 + 16 * lane))};
+  const uint32_t magic = magic_register<Bf16>();
+  uint32_t sw[128 / G];
 #pragma unroll
-    for (int gr = 0; gr < 128 / G; ++gr) sw[gr] = __ldg(reinterpret_cast<const uint32_t*>(in + kTileQ + 32 * gr + 4 * g));
+  for (int gr = 0; gr < 128 / G; ++gr) sw[gr] = __ldg(reinterpret_cast<const uint32_t*>(in + kTileQ + 32 * gr + 4 * g));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = nt * kTileN + 8 * h + g;
-      if (row >= N) continue;
-      const size_t at = ((size_t)b * N + row) * K + (size_t)kt * kTileK + 8 * t;
-      const uint32_t w[4] = {q[h].x, q[h].y, q[h].z, q[h].w};
+  for (int h = 0; h < 2; ++h) {
+    const int row = nt * kTileN + 8 * h + g;
+    if (row >= N) continue;
+    const size_t at = ((size_t)b * N + row) * K + (size_t)kt * kTileK + 8 * t;
+    const uint32_t w[4] = {q[h].x, q[h].y, q[h].z, q[h].w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t s2 = sw[j * 32 / G];
-        const float s = h == 0 ? __uint_as_float(s2 << 16) : __uint_as_float(s2 & 0xFFFF0000u);
-        uint32_t p[4];
-        decode_word<Bf16>(w[j], magic, p);
-        float v[8];
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t s2 = sw[j * 32 / G];
+      const float s = h == 0 ? __uint_as_float(s2 << 16) : __uint_as_float(s2 & 0xFFFF0000u);
+      uint32_t p[4];
+      decode_word<Bf16>(w[j], magic, p);
+      float v[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[2 * i] = __uint_as_float(p[i] << 16) * s;
-          v[2 * i + 1] = __uint_as_float(p[i] & 0xFFFF0000u) * s;
-        }
-        store8<TYPE>(out, at + 32 * j, v);
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(p[i] << 16) * s;
+        v[2 * i + 1] = __uint_as_float(p[i] & 0xFFFF0000u) * s;
       }
+      store8<TYPE>(out, at + 32 * j, v);
     }
+  }
   }
 }
 
-// One wave of resident CTAs at most: a warp walks its tiles.
-unsigned grid_for(long tiles) {
-  const long blocks = (tiles + kWarps - 1) / kWarps;
-  return (unsigned)(blocks < 148L * 8 ? blocks : 148L * 8);
+// CTAs for a warp per tile, `most` at most.  The quantiser takes all of them and the reader, whose warps walk their tiles, 32
+// per SM: with eight per SM, quantising and reading took 165 in place of 146 us (8 x 7168 x 2048, e4m3 to fp32) and reading
+// 13.0 in place of 12.2 (4096 x 7168, bf16).  A reader without the loop is slower (5 x 2045 x 1408, f16: 6.6 us, 5.75).
+unsigned grid_for(long tiles, long most) {
+  const long n = (tiles + kWarps - 1) / kWarps;
+  return (unsigned)(n < most ? n : most);
 }
 
 template <int TYPE, int G>
 cudaError_t run_quantize(const void* w, const float* bs, const void* given, long tiles, int N, int K, void* packed,
                          cudaStream_t stream) {
-  return launch_pdl(given ? quantize_kernel<TYPE, G, true> : quantize_kernel<TYPE, G, false>, dim3(grid_for(tiles)),
+  return launch_pdl(given ? quantize_kernel<TYPE, G, true> : quantize_kernel<TYPE, G, false>, dim3(grid_for(tiles, LONG_MAX)),
                     dim3(kWarps * 32), 0, stream, w, bs, reinterpret_cast<const uint16_t*>(given), (uint32_t)tiles, N, K,
                     reinterpret_cast<uint8_t*>(packed));
 }
@@ -297,7 +302,7 @@ cudaError_t pick_quantize(int group, const void* w, const float* bs, const void*
 }
 template <int TYPE, int G>
 cudaError_t run_dequantize(const void* packed, long tiles, int N, int K, void* out, cudaStream_t stream) {
-  return launch_pdl(dequantize_kernel<TYPE, G>, dim3(grid_for(tiles)), dim3(kWarps * 32), 0, stream,
+  return launch_pdl(dequantize_kernel<TYPE, G>, dim3(grid_for(tiles, 148 * 32)), dim3(kWarps * 32), 0, stream,
                     reinterpret_cast<const uint8_t*>(packed), (uint32_t)tiles, N, K, out);
 }
 template <int TYPE>

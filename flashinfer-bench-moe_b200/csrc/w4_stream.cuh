@@ -4,8 +4,8 @@
 //
 // Bytes in flight.  At 6.5 TB/s one SM takes 44 GB/s, and 1 to 2 us of latency under load ask for about 100 KB under way
 // per SM.  A ring belongs to one warp, which fills it itself: no producer warp, no empty barrier (a warp-wide sync orders
-// a slot's last read before its next copy).  A step is four tiles in one tensor copy.  More under way is slower (plain streaming of 1056-byte copies on a B200: 6.8 TB/s with 100 KB per SM, 6.5 with
-// 134, 5.6 with 200).
+// a slot's last read before its next copy).  A step is four tiles in one tensor copy.  More under way is slower (plain
+// streaming of 1056-byte copies on a B200: 6.8 TB/s with 100 KB per SM, 6.5 with 134, 5.6 with 200).
 //
 // Instructions.  86 cycles per two tiles and SM at that rate are 344 issue slots; the logic pipe takes two instructions a
 // cycle.  Decoding to pairs of 16-bit floats takes 7 logic instructions and 4 subtractions per word of eight weights, 242
