@@ -302,6 +302,21 @@ def test_linear_rows_captured(fbmoe_lib):
         assert torch.equal(y, e)
 
 
+def test_linear_offsets_past_32_bits(fbmoe_lib):
+    """More than 2^32 packed bytes in one matrix: its last rows, and its first."""
+    N, K, G = 1 << 20, 8192, 128
+    g = torch.Generator(device="cuda").manual_seed(2)
+    p = torch.randint(0, 256, (N // 16, K // 128, 1056), generator=g, device="cuda", dtype=torch.uint8)
+    scales = ((torch.rand((N // 16, K // 128, 16), generator=g, device="cuda") + 0.5) * 0.01).to(BF16)
+    p[..., 1024:] = scales.view(torch.uint8)
+    for T in (1, 9, 64):
+        x = torch.randn((T, K), generator=g, device="cuda").to(BF16)
+        y = fbmoe_lib.linear_w4(x, p)
+        for rows in (slice(0, 512), slice(N - 2000, N)):
+            v = fbmoe_lib.dequantize_w4(p[rows.start // 16:rows.stop // 16].contiguous(), dtype=F32).double()
+            check_linear(y[:, rows], x, v, G)
+
+
 # ------------------------------------------------------------------ the MoE layer
 class Case:
     def __init__(self, lib, T, E, offset, H, I, G1, G2, dtype, config, seed):
@@ -554,3 +569,71 @@ def test_moe_routes_as_route(fbmoe_lib, kind):
         got_idx = ws[at:at + 2048].view(torch.int32).view(64, 8)
         got_w = ws[at + 2048:at + 4096].view(torch.float32).view(64, 8)
         assert torch.equal(got_idx, idx) and torch.equal(got_w.view(torch.int32), w.view(torch.int32))
+
+
+# ------------------------------------------------------------------ calls at once
+def test_two_threads(fbmoe_lib):
+    """Two host threads, a stream each: layers and linears of either, many times."""
+    import threading
+    c = [Case(fbmoe_lib, T, 16, 0, 512, 256, 64, 64, BF16, "group", T) for T in (5, 33)]
+    p, _ = random_packed(300, 12288, 128, 4)
+    x = torch.randn((20, 12288), generator=torch.Generator().manual_seed(3)).to(BF16).cuda()
+    want, lin = [fbmoe_lib.forward_w4(*i.args()) for i in c], fbmoe_lib.linear_w4(x, p, 300)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(40):
+                    y, z = fbmoe_lib.forward_w4(*c[k].args()), fbmoe_lib.linear_w4(x, p, 300)
+                    s.synchronize()
+                    if not (torch.equal(y, want[k]) and torch.equal(z, lin)):
+                        wrong.append(k)
+        except Exception as e:  # reported below: an exception in a thread would pass unseen
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_layer_in_place(fbmoe_lib):
+    """The output may take the activations' place: they are read before the first output is written."""
+    c = Case(fbmoe_lib, 17, 16, 0, 512, 256, 64, 64, F16, "group", 3)
+    want = fbmoe_lib.forward_w4(*c.args())
+    x = c.x.clone()
+    args = list(c.args())
+    args[2] = x
+    y = fbmoe_lib.forward_w4(*args, out=x)
+    assert y.data_ptr() == x.data_ptr() and torch.equal(y, want)
+
+
+def test_beside_the_fp8_layer(fbmoe_lib, workloads):
+    """The fp8 layer (decode and prefill, which also use tensor memory) on one stream, 4-bit calls on another."""
+    w = workloads.make_weights(32, 77, "cuda")
+    inputs = [workloads.as_args(workloads.make_inputs(T, seed=T, device="cuda", E_local=32, weights=w)) for T in (16, 300)]
+    c = Case(fbmoe_lib, 33, 16, 0, 512, 256, 64, 64, BF16, "group", 8)
+    p, _ = random_packed(4096, 4096, 64, 4)
+    x = torch.randn((64, 4096), generator=torch.Generator().manual_seed(3)).to(BF16).cuda()
+    fp8 = [fbmoe_lib.forward(*i) for i in inputs]
+    want, lin = fbmoe_lib.forward_w4(*c.args()), fbmoe_lib.linear_w4(x, p)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        for i in inputs:
+            fbmoe_lib.forward(*i)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(15):
+        with torch.cuda.stream(a):
+            got += [(fbmoe_lib.forward(*i), r) for i, r in zip(inputs, fp8)]
+        with torch.cuda.stream(b):
+            got += [(fbmoe_lib.forward_w4(*c.args()), want), (fbmoe_lib.linear_w4(x, p), lin)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, r) for y, r in got)
+    fbmoe_lib.check_status()
