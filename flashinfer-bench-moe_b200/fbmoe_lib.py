@@ -531,7 +531,7 @@ def dequantize_w4(packed: torch.Tensor, n: int = None, dtype: torch.dtype = torc
     n, K, group = _w4_shape(packed, "packed", n)
     _require(dtype in _W4_TYPES and dtype != torch.float8_e4m3fn, "dtype must be bfloat16, float16 or float32")
     _require(packed.is_cuda, "packed must be a CUDA tensor")
-    out = torch.empty(packed.shape[:-3] + (n, K), dtype=dtype, device=packed.device)
+    out = packed.new_empty(packed.shape[:-3] + (n, K), dtype=dtype)
     if out.numel():
         _launch_on(packed.get_device(), "fbmoe_dequantize_w4", packed.data_ptr(), out.numel() // (n * K), n, K, group,
                    _W4_TYPES[dtype], out.data_ptr())
@@ -558,7 +558,7 @@ def linear_w4(x: torch.Tensor, weight: torch.Tensor, n: int = None, out: torch.T
     dev = x.get_device()
     _require(dev >= 0 and dev == weight.get_device(), "x and weight must be on one CUDA device")
     if out is None:
-        out = torch.empty((T, n), dtype=x.dtype, device=x.device)
+        out = x.new_empty((T, n))
         out_stride = n
     else:
         _require(out.dtype == x.dtype and tuple(out.shape) == (T, n) and out.get_device() == dev
@@ -621,7 +621,7 @@ def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2
     _require(dev >= 0 and dev == routing_logits.get_device() == routing_bias.get_device()
              == gemm1_weights.get_device() == gemm2_weights.get_device(), "all tensors must be on one CUDA device")
     if out is None:
-        out = torch.empty((T, H), dtype=x.dtype, device=x.device)
+        out = x.new_empty((T, H))
     else:
         _require(out.dtype == x.dtype and out.shape == (T, H) and out.is_contiguous() and out.get_device() == dev,
                  "out must be contiguous [T, H] in hidden_states' type on its device")
@@ -631,7 +631,7 @@ def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2
         if word:
             raise DeviceStatusError(word, "reported by an earlier forward_w4 on this device")
         nbytes = load_library().fbmoe_w4_workspace_size(T, H, I)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
         _launch_on(dev, "fbmoe_forward_w4", routing_logits.data_ptr(), routing_bias.data_ptr(), x.data_ptr(),
                    _W4_X_TYPES[x.dtype], gemm1_weights.data_ptr(), group1, gemm2_weights.data_ptr(), group2, T, H, I, E,
                    offset, routed_scaling_factor, out.data_ptr(), ws.data_ptr(), nbytes, sink)
