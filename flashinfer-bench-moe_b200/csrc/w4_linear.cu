@@ -31,7 +31,16 @@ namespace {
 
 constexpr int kWarps = 8;
 
-template <typename A, int G, int NT>
+// STREAM: the values take no place in the L1 cache, so that x stays there.
+template <bool STREAM>
+__device__ __forceinline__ uint4 load_values(const uint8_t* p) {
+  if (!STREAM) return __ldg(reinterpret_cast<const uint4*>(p));
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+template <typename A, int G, int NT, bool STREAM>
 __global__ void __launch_bounds__(kWarps * 32) tiles_kernel(const typename A::Raw* __restrict__ x, long ldx, int T,
                                                              const uint8_t* __restrict__ packed, int N, int K,
                                                              typename A::Raw* __restrict__ out, long ldo) {
@@ -43,8 +52,8 @@ __global__ void __launch_bounds__(kWarps * 32) tiles_kernel(const typename A::Ra
   float acc[NT][4] = {};
   for (int kt = warp; kt < kt_n; kt += kWarps) {
     const uint8_t* tile = packed + ((size_t)blockIdx.x * kt_n + kt) * tile_bytes(G);
-    const uint4 qlo = __ldg(reinterpret_cast<const uint4*>(tile + 16 * lane));
-    const uint4 qhi = __ldg(reinterpret_cast<const uint4*>(tile + 512 + 16 * lane));
+    const uint4 qlo = load_values<STREAM>(tile + 16 * lane);
+    const uint4 qhi = load_values<STREAM>(tile + 512 + 16 * lane);
     uint32_t sw[128 / G];
 #pragma unroll
     for (int gr = 0; gr < 128 / G; ++gr)
@@ -439,15 +448,17 @@ cudaError_t run_rows(const void* x, long ldx, int T, const void* packed, int N, 
 //   N x K          tiles to read    T = 8          T = 16         T = 64
 //   1024 x 4096    2048             3.2 / 5.5      4.0 / 5.6      6.1 / 7.0
 //   7168 x 2048    7168             4.6 / 7.2      7.0 / 7.5      18.0 / 9.9
-//   4096 x 7168    14336            10.7 / 9.9     11.4 / 10.0    32.3 / 12.4
-//   18432 x 7168   64512            24.4 / 22.4    31.8 / 22.5    98.6 / 27.6
-//   32001 x 7168   112056           31.5 / 43.8    49.6 / 43.9    170.7 / 52.6
+//   4096 x 7168    14336            7.8 / 9.9      11.4 / 10.0    32.3 / 12.4
+//   18432 x 7168   64512            19.3 / 22.4    31.8 / 22.5    98.6 / 27.6
+//   32001 x 7168   112056           28.5 / 43.8    49.6 / 43.9    170.7 / 52.6
 //   256 x 14336    1792             8.0 / 8.4      9.9 / 8.5      16.1 / 10.7
 // So rows_kernel takes more than 8 tokens if tiles_kernel would read more than 8192 tiles, or if K is so long that each of
 // its warps has twelve or more in a row.
+constexpr long kMany = 8192;
+long tiles_to_read(int T, int N, int K) { return ((long)(N - 1) / kTileN + 1) * (K / kTileK) * ((T + 15) / 16); }
 bool rows_pay(int T, int N, int K) {
-  const long kt = K / kTileK, tiles = ((long)(N - 1) / kTileN + 1) * kt * ((T + 15) / 16);
-  return T > 8 && (tiles > 8192 || kt >= 12 * kWarps);
+  const long kt = K / kTileK, tiles = tiles_to_read(T, N, K);
+  return T > 8 && (tiles > kMany || kt >= 12 * kWarps);
 }
 
 template <typename A, int G>
@@ -463,10 +474,15 @@ cudaError_t run_linear(const void* x, long ldx, int T, const void* packed, int N
     if (T <= 32) return run_rows<A, G, 32>(x, ldx, T, packed, N, K, out, ldo, stream);
     return run_rows<A, G, 64>(x, ldx, T, packed, N, K, out, ldo, stream);
   }
-  if (T <= 8)
-    return launch_pdl(tiles_kernel<A, G, 1>, dim3(nt), dim3(kWarps * 32), 0, stream, xp, ldx, T, wp, N, K, op, ldo);
-  return launch_pdl(tiles_kernel<A, G, 2>, dim3(nt, (unsigned)((T + 15) / 16)), dim3(kWarps * 32), 0, stream, xp, ldx,
-                    T, wp, N, K, op, ldo);
+  const dim3 grid(nt, (unsigned)((T + 15) / 16)), block(kWarps * 32);
+  if (T > 8) return launch_pdl(tiles_kernel<A, G, 2, false>, grid, block, 0, stream, xp, ldx, T, wp, N, K, op, ldo);
+  // Streamed, large matrices gain (4096 x 7168, 8 tokens: 10.6 us, 7.8; 18432 x 7168: 24.6, 19.6) and small ones lose (1024 x
+  // 4096, G = 32: 4.5, 5.2).  One token's x takes little of the cache, and its matrix may still lie in L2, from where
+  // streaming is slower (4096 x 7168, G = 32: up to 8.7 us, 9.7; from HBM 12.3, 9.9), so only a matrix of four times that
+  // size, 32 MB or more, is streamed for it (18432 x 7168, G = 32: 23.9, 20.6).
+  if (tiles_to_read(T, N, K) > (T == 1 ? 4 * kMany : kMany))
+    return launch_pdl(tiles_kernel<A, G, 1, true>, grid, block, 0, stream, xp, ldx, T, wp, N, K, op, ldo);
+  return launch_pdl(tiles_kernel<A, G, 1, false>, grid, block, 0, stream, xp, ldx, T, wp, N, K, op, ldo);
 }
 template <typename A>
 cudaError_t pick_linear(int group, const void* x, long ldx, int T, const void* packed, int N, int K, void* out,

@@ -235,7 +235,7 @@ def test_linear_rows_every_token_count(fbmoe_lib):
 
 
 @pytest.mark.parametrize("T,N,K", [(16, 8192, 2048), (16, 8193, 2048), (64, 2049, 2048), (64, 2048, 2048), (64, 16, 12160),
-                                   (64, 16, 12288), (8, 16, 12288)])
+                                   (64, 16, 12288), (8, 16, 12288), (8, 8192, 2048), (8, 8193, 2048), (1, 20000, 1024), (1, 40000, 2048)])
 def test_linear_on_both_sides_of_the_choice(fbmoe_lib, T, N, K):
     p, v = random_packed(N, K, 64, T + N)
     x = torch.randn((T, K), generator=torch.Generator().manual_seed(K)).to(BF16).cuda()
