@@ -3,10 +3,10 @@
 //   route as fbmoe_route; h = silu(x Wg^T) * (x Wu^T) for every (token, local expert) pair; out = sum over a token's
 //   pairs, in slot order, of weight * (h W2^T).
 //
-// W1's rows [0, I) are the linear half and [I, 2I) the silu half, as in fbmoe_forward.  x and h enter the products as
-// 16-bit integers with a power-of-two scale per 128 (x) or 32 (h) columns (w4_stream.cuh).
+// W1's rows [0, I) are the linear half and [I, 2I) the silu half, as in fbmoe_forward.  x enters its product as it is, h
+// as two bf16 numbers (w4_stream.cuh).
 //
-// route_kernel: one CTA per token; a warp routes it, all make its planes; also zeroes the layer kernel's counters.
+// route_kernel: a warp per token; also zeroes the layer kernel's counters.
 //
 // layer_kernel: one CTA per SM, working on units handed out by a ticket counter in the order
 //   up: (up to 8 rows of an expert; 32 MW pairs of W1 rows, two linear and two silu tiles side by side),
@@ -18,10 +18,9 @@
 //
 // The scheduler warp takes tickets ahead and waits for what a unit needs; 16 consumer warps, KW along K times MW along
 // the rows, stream the unit's tiles through their rings (w4_stream.cuh) and on into the next unit's; two finisher warps
-// add their partial sums in a fixed order, apply SwiGLU or the routing weight, store and report.  A unit takes an SM 3 to
-// 6 us at H = 7168, so phases and the end of the call are balanced to that; with a unit per warp or group of warps
-// (measured) they were not: 202 us in place of 165 at T = 64.  Every order of summation depends on the sizes and the
-// routing alone.
+// add their partial sums in a fixed order, apply SwiGLU or the routing weight, store and report.  A unit takes an SM 4 to
+// 8 us at H = 7168, so phases and the end of the call are balanced to that; with a unit per warp or group of warps they were
+// not, and T = 64 took a fifth longer.  Every order of summation depends on the sizes and the routing alone.
 #include "fbmoe.h"
 #include "fbmoe_launch.h"
 #include "moe_route.cuh"
@@ -49,7 +48,7 @@ struct Counters {
 };
 
 struct MoeLayout {
-  size_t counters, topk_idx, topk_w, xq, xs, hq, hs, pair_out, total;
+  size_t counters, topk_idx, topk_w, h, pair_out, total;
 };
 MoeLayout moe_layout(int T, int H, int I) {
   MoeLayout L;
@@ -62,96 +61,37 @@ MoeLayout moe_layout(int T, int H, int I) {
   L.counters = take(sizeof(Counters));
   L.topk_idx = take((size_t)T * kTopK * 4);
   L.topk_w = take((size_t)T * kTopK * 4);
-  L.xq = take((size_t)T * H * 2);                // planes of x
-  L.xs = take((size_t)T * (H / kTileK) * 4);     // their scales / 16
-  L.hq = take((size_t)T * kTopK * I * 2);        // planes of h, by pair
-  L.hs = take((size_t)T * kTopK * (I / 32) * 4);
+  L.h = take((size_t)T * kTopK * I * 4);         // [pair][two bf16 numbers][I]
   L.pair_out = take((size_t)T * kTopK * H * 4);    // [pair][H] fp32
   L.total = off;
   return L;
 }
 
-constexpr int kRouteThreads = 256;
-
-template <typename A>
-__device__ __forceinline__ float widen(typename A::Raw v) {
-  if constexpr (sizeof(A) == sizeof(Bf16) && A::kMagic == Bf16::kMagic) return __bfloat162float(v);
-  else return __half2float(v);
-}
-
-// Four consecutive values of a lane, 128 of a warp: their planes at the K position `dst`, their scale / 16 returned.
-__device__ __forceinline__ float make_planes(const float (&v)[4], uint8_t* dst) {
-  const int lane = threadIdx.x & 31;
-  float m = 0.0f;
-  bool bad = false;  // a NaN or an infinity
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    m = fmaxf(m, fabsf(v[i]));
-    bad |= !(fabsf(v[i]) <= 3.402823466e38f);
-  }
-  if (bad) m = INFINITY;
-#pragma unroll
-  for (int d = 16; d >= 1; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  const bool finite = m <= 3.402823466e38f;
-  const int e = plane_exponent(m);
-  uint32_t hi = 0, lo = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int k = finite ? plane_int(v[i], e) : 0;
-    hi |= (uint32_t)((k + 128) >> 8 & 0xff) << (8 * i);
-    lo |= (uint32_t)(k & 0xff) << (8 * i);
-  }
-  // an even lane holds elements 0..3 of an eight, the odd one next to it 4..7: bytes 0 4 1 5 | 2 6 3 7
-  const uint32_t ohi = __shfl_xor_sync(0xffffffffu, hi, 1), olo = __shfl_xor_sync(0xffffffffu, lo, 1);
-  const uint32_t order = lane & 1 ? 0x3726u : 0x5140u;
-  uint8_t* at = dst + (lane / 2 % 4) * 32 + (lane / 8) * 8 + (lane & 1) * 4;
-  *reinterpret_cast<uint32_t*>(at) = __byte_perm(hi, ohi, order);
-  *reinterpret_cast<uint32_t*>(at + 128) = __byte_perm(lo, olo, order);
-  return finite ? exp2_int(e) * 0.0625f : NAN;
-}
-
-template <typename A>
-__global__ void __launch_bounds__(kRouteThreads) route_kernel(const float* __restrict__ logits,
-                                                              const __nv_bfloat16* __restrict__ bias, float scale,
-                                                              const typename A::Raw* __restrict__ x, int H,
-                                                              int32_t* __restrict__ topk_idx, float* __restrict__ topk_w,
-                                                              uint8_t* __restrict__ xq, float* __restrict__ xs,
-                                                              Counters* __restrict__ counters) {
+__global__ void __launch_bounds__(32) route_kernel(const float* __restrict__ logits, const __nv_bfloat16* __restrict__ bias,
+                                                   float scale, int32_t* __restrict__ topk_idx, float* __restrict__ topk_w,
+                                                   Counters* __restrict__ counters) {
   __shared__ float wv[kExperts], ws[kExperts];
   __shared__ int wi[kExperts], sel[kTopK];
-  const int t = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int t = blockIdx.x;
   pdl_wait();
   pdl_trigger();
-  for (int i = t * kRouteThreads + threadIdx.x; i < (int)(sizeof(Counters) / 4); i += gridDim.x * kRouteThreads)
+  for (int i = t * 32 + threadIdx.x; i < (int)(sizeof(Counters) / 4); i += gridDim.x * 32)
     reinterpret_cast<uint32_t*>(counters)[i] = 0;
-  if (warp == 0) {
-    float l[8], b[8];
-    route_dev::load_logits8(logits, t, l);
-    route_dev::load_bias8(bias, b);
-    route_dev::route_token(l, t, b, scale, topk_idx, topk_w, wv, wi, ws, sel);
-    return;
-  }
-  const int kt_n = H / kTileK;
-  for (int kt = warp - 1; kt < kt_n; kt += kRouteThreads / 32 - 1) {
-    const uint2 r = *reinterpret_cast<const uint2*>(x + (size_t)t * H + kt * kTileK + 4 * lane);
-    const typename A::Raw* p = reinterpret_cast<const typename A::Raw*>(&r);
-    const float v[4] = {widen<A>(p[0]), widen<A>(p[1]), widen<A>(p[2]), widen<A>(p[3])};
-    const float sc = make_planes(v, xq + ((size_t)t * kt_n + kt) * kPlaneTile);
-    if (lane == 0) xs[(size_t)t * kt_n + kt] = sc;
-  }
+  float l[8], b[8];
+  route_dev::load_logits8(logits, t, l);
+  route_dev::load_bias8(bias, b);
+  route_dev::route_token(l, t, b, scale, topk_idx, topk_w, wv, wi, ws, sel);
 }
 
 struct LayerArgs {
   CUtensorMap map1, map2;  // W1, W2
   int T, H, I, E, offset;
   int kw1[2], kw2[2];    // consumer warps along K of an up / down unit: for small calls, for large ones
-  int depth;             // steps of a ring
   const int32_t* topk_idx;
   const float* topk_w;
-  const uint8_t* xq;
-  const float* xs;
-  uint8_t* hq;
-  float *hs, *pair_out;
+  const void* x;
+  __nv_bfloat16* h;
+  float* pair_out;
   Counters* counters;
   void* out;
   uint32_t* sink;
@@ -175,7 +115,7 @@ __device__ __forceinline__ int kind_of(const Unit& u) { return u.block >> 28; }
 
 struct Shared {
   unsigned long long mask[kExperts];  // tokens of each local expert
-  uint64_t ring_full[kStreamWarps][kMaxDepth];
+  uint64_t ring_full[kStreamWarps][kDepth];
   uint64_t known[kQueue], go[kQueue], done[kQueue];  // a queue slot's unit is there; may be begun; is finished
   uint64_t part_full[2], part_empty[2];
   Unit unit[kQueue];
@@ -240,6 +180,7 @@ __device__ __forceinline__ void build_lists(const LayerArgs& a, Shared& s) {
   __syncthreads();
 }
 
+constexpr float kMaxBf16 = 3.38953139e38f;  // an h beyond it would round to infinity
 __device__ __forceinline__ float swiglu(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
 
 // What a consumer warp has of a unit: K positions [k0, k0 + steps) of four row tiles.
@@ -268,121 +209,91 @@ __device__ __forceinline__ uint32_t row_groups(const LayerArgs& a, const Unit& u
 constexpr int tile_words(int group) { return tile_bytes(group) / 8; }
 template <int G1, int G2>
 struct Stream {
-  Ring ring;
-  const CUtensorMap* map;
-  int x, row, matrix;
-  int left;        // steps of the unit being issued that are still to be issued
-  uint32_t words;  // 8-byte elements of a tile
-  uint64_t policy;
-  uint32_t seq;    // units begun
-  bool more;
+  Ring<step_bytes(G1 < G2 ? G1 : G2)> ring;
+  int x, row;
+  uint32_t unit;  // the local expert, and whether it is an up unit in bit 8
+  int left;       // steps of the unit being issued that are still to be issued
+  uint32_t seq;   // units begun; kNoMore: there are none left
+  static constexpr uint32_t kNoMore = 1u << 31;
 
-  __device__ __forceinline__ void step() {
-    ring.issue(map, x, row, 0, matrix, words * 32, policy);
+  __device__ __forceinline__ void step(const LayerArgs& a) {
+    const bool up = unit >> 8;
+    const int words = up ? tile_words(G1) : tile_words(G2);
+    ring.issue(up ? &a.map1 : &a.map2, x, row, unit & 0xff, words * 32);
     x += words;
     --left;
   }
   // Issue steps while the ring has room.
   __device__ __forceinline__ void fill(const LayerArgs& a, Shared& s) {
-    if (left > 0 && ring.free == 1) {  // the usual case: the step just released
-      step();
-      return;
-    }
-    while (ring.free > 0) {
-      if (left == 0) {
-        // the next unit, if it is known
-        if (!more || !__all_sync(0xffffffffu, Ring::test(smem_u32(&s.known[seq % kQueue]), seq / kQueue & 1))) return;
-        const Unit u = s.unit[seq % kQueue];
-        ++seq;
-        const int kind = kind_of(u);
-        more = kind == kUp || kind == kDown;
-        const uint32_t group = row_group(s, u, threadIdx.x / 32);
-        if (!more || group >= row_groups(a, u)) continue;
-        const Span w = span_of(a, s, kind == kUp);
-        words = kind == kUp ? tile_words(G1) : tile_words(G2);
-        map = kind == kUp ? &a.map1 : &a.map2;
-        x = w.k0 * words;
-        row = kind == kUp ? 2 * group : 4 * group;
-        matrix = block_expert(u.block);
-        left = w.steps;
+    while (!ring.full()) {
+      if (left > 0) {
+        step(a);
         continue;
       }
-      step();
+      // the next unit, if it is known
+      if (seq >= kNoMore || !__all_sync(0xffffffffu, ring.test(smem_u32(&s.known[seq % kQueue]), seq / kQueue & 1))) return;
+      const Unit u = s.unit[seq % kQueue];
+      ++seq;
+      const int kind = kind_of(u);
+      if (kind != kUp && kind != kDown) {
+        seq |= kNoMore;
+        return;
+      }
+      const uint32_t group = row_group(s, u, threadIdx.x / 32);
+      if (group >= row_groups(a, u)) continue;
+      const Span w = span_of(a, s, kind == kUp);
+      x = w.k0 * (kind == kUp ? tile_words(G1) : tile_words(G2));
+      row = kind == kUp ? 2 * group : 4 * group;
+      unit = block_expert(u.block) | (kind == kUp) << 8;
+      left = w.steps;
     }
   }
 };
 
-// The lane's places in the planes and scales of up to 4 NT tokens of a task (rows that are not there read the first
-// one's: their sums are not used), from K position k0 on.
-template <int NT, bool FINE>
+// The lane's places in the activations of a task's rows from K position k0 on, columns as tile_product takes them (rows
+// that are not there read the first one's: their sums are not used).  The loads are plain ones: x may be the call's output,
+// which is written once no unit reads it any more, and h is written while the kernel runs.
+template <int NT, bool PAIR>
 struct Places {
-  const uint8_t* q[NT];
-  const float* s[NT];
+  static constexpr int NC = PAIR ? NT : 1;
+  const uint8_t* p[NC];
 
-  __device__ __forceinline__ void at(const uint8_t* planes, const float* scales, int kt_n, int k0, const Shared& s_,
-                                     uint32_t block, bool by_pair) {
+  __device__ __forceinline__ void at(const void* base, int width, int k0, const Shared& s, uint32_t block) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int pos = block_pos(block), rows = block_rows_of(block);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int rq = 4 * n + (g >> 1), rs = 4 * n + t;
-      int pq = s_.pairs[pos + (rq < rows ? rq : 0)], ps = s_.pairs[pos + (rs < rows ? rs : 0)];
-      if (!by_pair) {
-        pq /= kTopK;
-        ps /= kTopK;
-      }
-      q[n] = planes + ((size_t)pq * kt_n + k0) * kPlaneTile + (g & 1) * 128 + t * 32;
-      s[n] = scales + ((size_t)ps * kt_n + k0) * (FINE ? 4 : 1);
+    for (int n = 0; n < NC; ++n) {
+      const int r = PAIR ? 4 * n + (g >> 1) : 4 * (g & 1) + (g >> 1);
+      const int pair = s.pairs[pos + (r < rows ? r : 0)];
+      const size_t row = PAIR ? 2 * pair + (g & 1) : pair / kTopK;
+      p[n] = reinterpret_cast<const uint8_t*>(base) + (row * width + (size_t)k0 * kTileK + 8 * t) * 2;
     }
   }
-  // The current K position's words 2j, 2j + 1, and its scales.  x is constant while the kernel runs, h is not.
-  __device__ __forceinline__ void load(Columns<NT, FINE>& c, int j) const {
+  // The current K position's words j.
+  __device__ __forceinline__ void load(Columns<NC>& c, int j) const {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint4* p = reinterpret_cast<const uint4*>(q[n]) + j;
-      const uint4 u = FINE ? *p : __ldg(p);
-      c.b[n][2 * j] = make_uint2(u.x, u.y);
-      c.b[n][2 * j + 1] = make_uint2(u.z, u.w);
-    }
-  }
-  __device__ __forceinline__ void load_scales(Columns<NT, FINE>& c) const {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if constexpr (FINE) {
-        const float4 f = *reinterpret_cast<const float4*>(s[n]);
-        c.s[n][0] = f.x;
-        c.s[n][1] = f.y;
-        c.s[n][2] = f.z;
-        c.s[n][3] = f.w;
-      } else {
-        c.s[n][0] = __ldg(s[n]);
-      }
-    }
+    for (int n = 0; n < NC; ++n) c.v[n][j] = *reinterpret_cast<const uint4*>(p[n] + 64 * j);
   }
   __device__ __forceinline__ void advance() {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      q[n] += kPlaneTile;
-      s[n] += FINE ? 4 : 1;
-    }
+    for (int n = 0; n < NC; ++n) p[n] += kTileK * 2;
   }
 };
 
 // A consumer warp's part of a unit of up to 4 NT rows, its sums left in `part` ([n][tiles 0 1, tiles 2 3][lane][tile, 8 i]:
 // row 8 i + g of the tile, token 4n + t).
-template <int G, int NT, bool UP, typename S, typename Wait>
+template <typename A, int G, int NT, bool UP, typename S, typename Wait>
 __device__ __forceinline__ bool consume(const LayerArgs& a, Shared& s, S& st, const Unit& u, const Span& w, float* part,
                                         const Wait& free_part) {
   const int lane = threadIdx.x & 31, g = lane >> 2;
-  const uint32_t flip = flip_register();
+  const uint32_t magic = magic_register<A>();
   float acc[4][NT][2] = {};
   if (row_group(s, u, threadIdx.x / 32) < row_groups(a, u)) {
     Places<NT, !UP> at;
-    at.at(UP ? a.xq : a.hq, UP ? a.xs : a.hs, (UP ? a.H : a.I) / kTileK, w.k0, s, u.block, !UP);
-    Columns<NT, !UP> x;
-    at.load(x, 0);
-    at.load(x, 1);
-    at.load_scales(x);
+    at.at(UP ? a.x : a.h, UP ? a.H : a.I, w.k0, s, u.block);
+    Columns<UP ? 1 : NT> x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) at.load(x, j);
     auto keep = [](int) {};
     // the last tile's product is followed word by word by the loads of the next K position's columns: no registers of
     // their own, and their latency passes under the next wait and the first tile
@@ -391,12 +302,11 @@ __device__ __forceinline__ bool consume(const LayerArgs& a, Shared& s, S& st, co
     for (int left = w.steps; left > 0; --left) {
       if (left > 1) at.advance();  // the last one is read twice
       st.ring.wait(&s.abort);
-      const uint32_t words = st.ring.got + 16 * lane, scales = st.ring.got + 4 * g;
-      tile_product<G, NT, !UP, 0>(words, scales, x, flip, acc[0], keep);
-      tile_product<G, NT, !UP, tile_bytes(G)>(words, scales, x, flip, acc[1], keep);
-      tile_product<G, NT, !UP, 2 * tile_bytes(G)>(words, scales, x, flip, acc[2], keep);
-      tile_product<G, NT, !UP, 3 * tile_bytes(G)>(words, scales, x, flip, acc[3], reload);
-      at.load_scales(x);
+      const uint32_t slot = st.ring.slot(), words = slot + 16 * lane, scales = slot + 4 * g;
+      tile_product<A, G, NT, !UP, 0>(words, scales, x, magic, acc[0], keep);
+      tile_product<A, G, NT, !UP, tile_bytes(G)>(words, scales, x, magic, acc[1], keep);
+      tile_product<A, G, NT, !UP, 2 * tile_bytes(G)>(words, scales, x, magic, acc[2], keep);
+      tile_product<A, G, NT, !UP, 3 * tile_bytes(G)>(words, scales, x, magic, acc[3], reload);
       st.ring.release();
       st.fill(a, s);
     }
@@ -428,31 +338,17 @@ __device__ __forceinline__ void sum_parts(const float* part, int kw, int n, floa
 // 32 columns of h: v holds the linear tiles, then the silu tiles.
 __device__ __forceinline__ void finish_up(const LayerArgs& a, const Shared& s, uint32_t block, int n, uint32_t group,
                                           const float (&v)[8]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float h[4], m = 0.0f;  // columns 8 i + g
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    h[i] = swiglu(v[4 + i], v[i]);
-    m = fmaxf(m, fabsf(h[i]));
-    bad |= !(fabsf(h[i]) <= 3.402823466e38f);
-  }
-  if (bad) m = INFINITY;
-#pragma unroll
-  for (int d = 16; d >= 4; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  const bool finite = m <= 3.402823466e38f;
-  const int e = plane_exponent(m), r = 4 * n + t;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, r = 4 * n + t;
   if (r >= block_rows_of(block)) return;
-  const size_t pair = s.pairs[block_pos(block) + r];
-  // column 8 i + g of these 32: eight i, element g, which is byte g / 4 + g % 4 * 2 of its eight
-  uint8_t* dst = a.hq + (pair * (a.I / kTileK) + group / 4) * kPlaneTile + group % 4 * 8 + (g >> 2) + (g & 3) * 2;
+  __nv_bfloat16* dst = a.h + (size_t)s.pairs[block_pos(block) + r] * 2 * a.I + group * kUpSpan + g;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int q = finite ? plane_int(h[i], e) : 0;
-    dst[32 * i] = (uint8_t)((q + 128) >> 8);
-    dst[32 * i + 128] = (uint8_t)q;
+  for (int i = 0; i < 4; ++i) {  // columns 8 i + g
+    const float h = swiglu(v[4 + i], v[i]);
+    const bool finite = fabsf(h) <= FLT_MAX;
+    const __nv_bfloat16 hi = __float2bfloat16_rn(finite ? fminf(fmaxf(h, -kMaxBf16), kMaxBf16) : h);
+    dst[8 * i] = hi;
+    dst[8 * i + a.I] = __float2bfloat16_rn(finite ? h - __bfloat162float(hi) : 0.0f);
   }
-  if (g == 0) a.hs[pair * (a.I / 32) + group] = finite ? exp2_int(e) * 0.0625f : NAN;
 }
 
 // 64 outputs of each pair, weighted.
@@ -494,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) layer_kernel(const __grid_constan
   constexpr int kSlot = step_bytes(G1 < G2 ? G1 : G2);
   Shared& s = *reinterpret_cast<Shared*>(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x < kStreamWarps * kMaxDepth) mbar_init(&s.ring_full[0][0] + threadIdx.x, 1);
+  if (threadIdx.x < kStreamWarps * kDepth) mbar_init(&s.ring_full[0][0] + threadIdx.x, 1);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kQueue; ++i) {
       mbar_init(&s.known[i], 1);
@@ -512,8 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1) layer_kernel(const __grid_constan
   pdl_trigger();
   build_lists(a, s);  // synchronises the CTA
   if (threadIdx.x < 2) {
-    // Longer runs along K per warp where that still leaves four units per SM (T = 64, a quarter of the experts: 166 us with
-    // the shorter ones, 157 with the longer), shorter ones otherwise (T = 1, H 2048, I 768: 23 us, 29 with the longer).
+    // Longer runs along K per warp where that still leaves four units per SM (T = 64, a quarter of the experts: 207 us with
+    // the shorter ones, 195 with the longer), shorter ones otherwise (T = 33, H 2048, I 768: 61 us, 65.5 with the longer).
     const int* kw = threadIdx.x ? a.kw2 : a.kw1;
     const int groups = threadIdx.x ? a.H / kDownSpan : a.I / kUpSpan, mw = kStreamWarps / kw[1];
     (threadIdx.x ? s.kw2 : s.kw1) = s.n_blocks * ((groups + mw - 1) / mw) >= 4 * (int)gridDim.x ? kw[1] : kw[0];
@@ -624,11 +520,9 @@ __global__ void __launch_bounds__(kThreads, 1) layer_kernel(const __grid_constan
   } else {
     const Span up = span_of(a, s, true), down = span_of(a, s, false);
     Stream<G1, G2> st;
-    st.ring.init(smem_u32(parts + 2 * kParts) + warp * a.depth * kSlot, smem_u32(s.ring_full[warp]), kSlot, a.depth);
-    st.policy = l2_policy_evict_first();
+    st.ring.init(smem_u32(parts + 2 * kParts) + warp * kDepth * kSlot, smem_u32(s.ring_full[warp]));
     st.left = 0;
     st.seq = 0;
-    st.more = true;
     uint32_t n = 0;
     for (uint32_t seq = 0;; ++seq) {
       const int slot = seq % kQueue;
@@ -647,11 +541,11 @@ __global__ void __launch_bounds__(kThreads, 1) layer_kernel(const __grid_constan
         auto free_part = [&] { return wait(&s.part_empty[b], parity); };
         bool ok;
         if (kind == kUp) {
-          if (block_rows_of(u.block) <= 4) ok = consume<G1, 1, true>(a, s, st, u, up, part, free_part);
-          else ok = consume<G1, 2, true>(a, s, st, u, up, part, free_part);
+          if (block_rows_of(u.block) <= 4) ok = consume<A, G1, 1, true>(a, s, st, u, up, part, free_part);
+          else ok = consume<A, G1, 2, true>(a, s, st, u, up, part, free_part);
         } else {
-          if (block_rows_of(u.block) <= 4) ok = consume<G2, 1, false>(a, s, st, u, down, part, free_part);
-          else ok = consume<G2, 2, false>(a, s, st, u, down, part, free_part);
+          if (block_rows_of(u.block) <= 4) ok = consume<Bf16, G2, 1, false>(a, s, st, u, down, part, free_part);
+          else ok = consume<Bf16, G2, 2, false>(a, s, st, u, down, part, free_part);
         }
         if (!ok) break;
         __syncwarp();
@@ -661,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) layer_kernel(const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.done[slot]);
     }
-    if (!st.ring.drain(a.depth) && lane == 0) atomicOr(&a.counters->status, kStatusTimeoutDrain);
+    if (!st.ring.drain() && lane == 0) atomicOr(&a.counters->status, kStatusTimeoutDrain);
   }
   __syncthreads();
   if (threadIdx.x == 0 && s.abort) atomicOr(&a.counters->status, kStatusTimeoutEpilogue);
@@ -705,7 +599,9 @@ bool map_weights(CUtensorMap* map, const uint8_t* base, int k_tiles, int words, 
 template <typename A, int G1, int G2>
 cudaError_t run_layer(const MoeArgs& m, const MoeLayout& L, int sms) {
   static DeviceFlags smem_set;
-  cudaError_t e = set_max_dynamic_smem(layer_kernel<A, G1, G2>, kSmemMax, smem_set);
+  constexpr int kSmem = (int)kFixedSmem + 2 * kStreamWarps * kPart * 4 + kStreamWarps * kDepth * step_bytes(G1 < G2 ? G1 : G2);
+  static_assert(kSmem <= kSmemMax, "shared memory over the per-CTA limit");
+  cudaError_t e = set_max_dynamic_smem(layer_kernel<A, G1, G2>, kSmem, smem_set);
   if (e != cudaSuccess) return e;
   alignas(64) LayerArgs a;
   if (!map_weights(&a.map1, m.w1, m.H / kTileK, tile_words(G1), m.I / kTileN, 2, m.E, 2) ||
@@ -716,20 +612,14 @@ cudaError_t run_layer(const MoeArgs& m, const MoeLayout& L, int sms) {
   a.I = m.I;
   a.E = m.E;
   a.offset = m.offset;
-  constexpr int kSlot = step_bytes(G1 < G2 ? G1 : G2);
   for (int i = 0; i < 2; ++i) {
     a.kw1[i] = k_groups(m.H / kTileK, 2 + 2 * i);
     a.kw2[i] = k_groups(m.I / kTileK, 2 + 2 * i);
   }
-  constexpr int kFixed = (int)kFixedSmem + 2 * kStreamWarps * kPart * 4;
-  a.depth = (kSmemMax - kFixed) / (kStreamWarps * kSlot);
-  if (a.depth > kMaxDepth) a.depth = kMaxDepth;
   a.topk_idx = reinterpret_cast<const int32_t*>(m.ws + L.topk_idx);
   a.topk_w = reinterpret_cast<const float*>(m.ws + L.topk_w);
-  a.xq = m.ws + L.xq;
-  a.xs = reinterpret_cast<const float*>(m.ws + L.xs);
-  a.hq = m.ws + L.hq;
-  a.hs = reinterpret_cast<float*>(m.ws + L.hs);
+  a.x = m.x;
+  a.h = reinterpret_cast<__nv_bfloat16*>(m.ws + L.h);
   a.pair_out = reinterpret_cast<float*>(m.ws + L.pair_out);
   a.counters = reinterpret_cast<Counters*>(m.ws + L.counters);
   a.out = m.out;
@@ -737,8 +627,7 @@ cudaError_t run_layer(const MoeArgs& m, const MoeLayout& L, int sms) {
   const bool expire = test_expire_grid_wait();
   a.wait_ns = expire ? kTestGridWaitNs : kWaitBudgetNs;
   a.extra = expire ? 1u : 0u;
-  return launch_pdl(layer_kernel<A, G1, G2>, dim3(sms), dim3(kThreads), (size_t)kFixed + (size_t)a.depth * kStreamWarps * kSlot,
-                    m.stream, a);
+  return launch_pdl(layer_kernel<A, G1, G2>, dim3(sms), dim3(kThreads), kSmem, m.stream, a);
 }
 template <typename A, int G1>
 cudaError_t pick_layer(const MoeArgs& m, const MoeLayout& L, int sms) {
@@ -749,11 +638,10 @@ cudaError_t pick_layer(const MoeArgs& m, const MoeLayout& L, int sms) {
 template <typename A>
 cudaError_t run_moe(const MoeArgs& m) {
   const MoeLayout L = moe_layout(m.T, m.H, m.I);
-  cudaError_t e = launch_pdl(route_kernel<A>, dim3(m.T), dim3(kRouteThreads), 0, m.stream, m.logits,
+  cudaError_t e = launch_pdl(route_kernel, dim3(m.T), dim3(32), 0, m.stream, m.logits,
                              reinterpret_cast<const __nv_bfloat16*>(m.bias), m.scale,
-                             reinterpret_cast<const typename A::Raw*>(m.x), m.H,
-                             reinterpret_cast<int32_t*>(m.ws + L.topk_idx), reinterpret_cast<float*>(m.ws + L.topk_w), m.ws + L.xq,
-                             reinterpret_cast<float*>(m.ws + L.xs), reinterpret_cast<Counters*>(m.ws + L.counters));
+                             reinterpret_cast<int32_t*>(m.ws + L.topk_idx), reinterpret_cast<float*>(m.ws + L.topk_w),
+                             reinterpret_cast<Counters*>(m.ws + L.counters));
   if (e != cudaSuccess) return e;
   const int sms = num_sms_of_current_device();
   if (m.group1 == 32) return pick_layer<A, 32>(m, L, sms);

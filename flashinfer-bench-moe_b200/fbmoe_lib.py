@@ -593,7 +593,8 @@ def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2
     """The fused MoE layer for at most 64 tokens on packed 4-bit weights: ``hidden_states`` [T, H] bfloat16 or float16,
     ``gemm1_weights`` E_local packed [2I, H] matrices (rows [0, I) the linear half, [I, 2I) the silu half),
     ``gemm2_weights`` E_local packed [H, I] matrices, routing as ``forward``; returns [T, H] in hidden_states' type
-    (``out`` may be hidden_states itself).
+    (``out`` may be hidden_states itself).  Activations are taken as they are, sums are fp32, the SwiGLU output is held as
+    two bf16 numbers (within 2^-16 of itself) and the result is rounded once.
     The workspace is allocated per call, so calls may overlap and captured graphs share nothing.  Device-side errors
     (a bounded wait that expired) raise DeviceStatusError as in ``forward``: at a later call on the device or at
     check_status(), or for this call with ``sync_status`` (or FBMOE_SYNC_STATUS=1)."""

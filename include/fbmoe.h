@@ -338,8 +338,8 @@ FBMOE_API int fbmoe_linear_w4(const void* x, int64_t x_stride, int type, int T, 
  * fbmoe_forward (256 experts, top-8), hidden_states and out [T, H] of `type`
  * (FBMOE_BF16 or FBMOE_F16), gemm1_weights E_local packed [2I, H] matrices (rows
  * [0, I) the linear half, [I, 2I) the silu half), gemm2_weights E_local packed
- * [H, I] matrices; H and I multiples of 128; sums in fp32, the result rounded
- * once.  Pointers 16-byte aligned; workspace >= fbmoe_w4_workspace_size(T, H, I)
+ * [H, I] matrices; H and I multiples of 128; sums in fp32, the intermediate held
+ * as two bf16 numbers (within 2^-16 of itself), the result rounded once.  Pointers 16-byte aligned; workspace >= fbmoe_w4_workspace_size(T, H, I)
  * bytes, 256-byte aligned; calls that may overlap need a workspace each.  A bounded
  * wait that expires sets the status word at the workspace's start (the bits of
  * fbmoe_read_status) and stores it to status_sink (device-accessible, e.g. pinned host memory;
