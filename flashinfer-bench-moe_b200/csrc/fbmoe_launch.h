@@ -164,6 +164,8 @@ uint32_t* status_sink_for(const void* workspace);
 // kTestGridWaitNs, so every CTA's bounded wait expires and reports
 // kStatusTimeoutEpilogue without any fault.
 bool test_expire_grid_wait();
+// The same hook set to 2: the 4-bit linear layer's waits have a budget of kTestGridWaitNs and nothing is missing.
+bool test_short_waits();
 constexpr uint64_t kTestGridWaitNs = 2000000ull;
 
 // GEMM1 + SwiGLU for blocks of 128 rows with the tokens as the MMA M operand.

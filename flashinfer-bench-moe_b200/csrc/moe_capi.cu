@@ -193,7 +193,8 @@ uint32_t* status_sink_for(const void* workspace) {
 }
 
 static std::atomic<int> g_test_expire{0};
-bool test_expire_grid_wait() { return g_test_expire.load(std::memory_order_relaxed) != 0; }
+bool test_expire_grid_wait() { return g_test_expire.load(std::memory_order_relaxed) == 1; }
+bool test_short_waits() { return g_test_expire.load(std::memory_order_relaxed) != 0; }
 
 }  // namespace fbmoe
 
@@ -504,7 +505,7 @@ int fbmoe_set_status_sink(const void* workspace, uint32_t* sink) {
 }
 
 int fbmoe_test_expire_grid_wait(int enable) {
-  g_test_expire.store(enable ? 1 : 0, std::memory_order_relaxed);
+  g_test_expire.store(enable == 0 || enable == 2 ? enable : 1, std::memory_order_relaxed);
   return FBMOE_OK;
 }
 

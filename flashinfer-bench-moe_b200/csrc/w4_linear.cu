@@ -166,7 +166,7 @@ template <typename A, int G, int NP>
 __global__ void __launch_bounds__(kRowsThreads, 1)
     rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
                 const __grid_constant__ CUtensorMap map_x, int T, int N, int kt_n,
-                int splits, typename A::Raw* __restrict__ out, long ldo) {
+                int splits, typename A::Raw* __restrict__ out, long ldo, uint64_t wait_ns) {
   using S = RowsSmem<G, NP>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -199,11 +199,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_wait();  // every thread: a role's limit counts from here, however long the predecessor takes
   pdl_trigger();
   const uint32_t tmem = *tmem_at;
   // A wait that gives up raises `abort`, and every role ends; the outputs are then written as NaN.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (mbar_wait(bar, parity, abort, kWaitBudgetNs)) return true;
+    if (mbar_wait(bar, parity, abort, wait_ns)) return true;
     *abort = 1;
     return false;
   };
@@ -217,7 +218,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   for (int i = 0; i < kMine / 2; ++i) acc[i] = 0;
 
   if (warp == 0 || warp == 3) {  // copies of the matrix; of x
-    pdl_wait();
     fence_proxy_async_global();
     const uint64_t policy = l2_policy_evict_first();
     // One after the other through `stages` places.
@@ -439,7 +439,7 @@ cudaError_t run_rows(const void* x, long ldx, int T, const void* packed, int N, 
   cfg.attrs = attr;
   cfg.numAttrs = splits > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, rows_kernel<A, G, NP>, map_w, map_s, map_x, T, N, kt, splits,
-                            reinterpret_cast<typename A::Raw*>(out), ldo);
+                            reinterpret_cast<typename A::Raw*>(out), ldo, test_short_waits() ? kTestGridWaitNs : kWaitBudgetNs);
 }
 
 // Which kernel, by how much there is to spread over the SMs.  tiles_kernel reads the matrix once per 16 tokens and starts and

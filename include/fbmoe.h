@@ -206,7 +206,8 @@ FBMOE_API int fbmoe_decode_launch_mode(void);
 /* Test hook: while `enable` is non-zero the decode kernel's grid-arrival wait
  * waits for one arrival that never comes, with a 2 ms budget, so every CTA's
  * bounded wait expires, sets status bit 2 and returns without writing its part
- * of the output.  Lets tests exercise the error path without any device fault. */
+ * of the output.  Lets tests exercise the error path without any device fault.
+ * 2: nothing is missing, and the waits of fbmoe_linear_w4 have that budget. */
 FBMOE_API int fbmoe_test_expire_grid_wait(int enable);
 
 /* Stage timing for measurement: after fbmoe_profile_begin(n), the next n
