@@ -301,7 +301,10 @@ __device__ __forceinline__ bool consume(const LayerArgs& a, Shared& s, S& st, co
 #pragma unroll 1
     for (int left = w.steps; left > 0; --left) {
       if (left > 1) at.advance();  // the last one is read twice
-      st.ring.wait(&s.abort);
+      if (!st.ring.wait()) {
+        s.abort = 1;
+        return false;
+      }
       const uint32_t slot = st.ring.slot(), words = slot + 16 * lane, scales = slot + 4 * g;
       tile_product<A, G, NT, !UP, 0>(words, scales, x, magic, acc[0], keep);
       tile_product<A, G, NT, !UP, tile_bytes(G)>(words, scales, x, magic, acc[1], keep);
@@ -555,10 +558,18 @@ __global__ void __launch_bounds__(kThreads, 1) layer_kernel(const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.done[slot]);
     }
-    if (!st.ring.drain() && lane == 0) atomicOr(&a.counters->status, kStatusTimeoutDrain);
+    if (!st.ring.drain() && lane == 0) {
+      s.abort = 1;
+      atomicOr(&a.counters->status, kStatusTimeoutDrain);
+    }
   }
   __syncthreads();
-  if (threadIdx.x == 0 && s.abort) atomicOr(&a.counters->status, kStatusTimeoutEpilogue);
+  if (s.abort) {
+    if (threadIdx.x == 0) atomicOr(&a.counters->status, kStatusTimeoutEpilogue);
+    // All outputs become NaN.  A CTA that combines after this found all units finished, and writes right values over it.
+    typename A::Raw* out = reinterpret_cast<typename A::Raw*>(a.out);
+    for (long i = threadIdx.x; i < (long)a.T * a.H; i += kThreads) out[i] = A::of(__uint_as_float(0x7FC00000u));
+  }
   __syncthreads();
   if (threadIdx.x == 0) forward_status_to_sink(&a.counters->status, a.sink);
 }

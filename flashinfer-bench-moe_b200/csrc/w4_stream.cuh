@@ -36,14 +36,12 @@ __host__ __device__ constexpr int step_bytes(int group) { return kStepTiles * ti
 
 // ---------------------------------------------------------------- ring ------
 // One warp's ring.  Steps are issued and consumed in order.  Slots and barriers are shared-memory addresses.  Its waits
-// are for its own copies, which land by themselves; one that gives up all the same raises `abort` and closes the ring:
-// nothing more is issued, and the warp goes on over whatever the slots hold until it meets one of the waits that look at
-// `abort`.  The caller reports the call as failed.
+// are for its own copies, which land by themselves; if one gives up all the same, the warp ends its role with the unit
+// unfinished, and the caller reports the call as failed.
 template <int SLOT>
 struct Ring {
-  static constexpr int kClosed = 1 << 30;
   uint32_t slots, bars;
-  int put, got;  // steps issued, steps consumed (put far above got: closed)
+  int put, got;  // steps issued, steps consumed
 
   __device__ __forceinline__ void init(uint32_t slots_, uint32_t barriers) {
     slots = slots_;
@@ -78,14 +76,10 @@ struct Ring {
         : "memory");
     return ok != 0;
   }
-  // Wait for the next step's tiles.
-  __device__ __forceinline__ void wait(volatile int* abort) {
+  // Wait for the next step's tiles; false, for all lanes, when the limit runs out.
+  __device__ __forceinline__ bool wait() const {
     const uint32_t bar = bars + got % kDepth * 8, parity = got / kDepth & 1;
-    if (test(bar, parity)) return;
-    if (put - got <= kDepth && !wait_slow(bar, parity)) {
-      *abort = 1;
-      put += kClosed;
-    }
+    return __all_sync(0xffffffffu, test(bar, parity)) || __all_sync(0xffffffffu, wait_slow(bar, parity));
   }
   static __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity) {
     const uint64_t t0 = globaltimer_ns();
@@ -102,7 +96,6 @@ struct Ring {
   // Before the CTA ends no copy may be under way: those issued and not consumed are waited for (none after a complete
   // call).  False when the limit runs out.
   __device__ __forceinline__ bool drain() {
-    if (put - got > kDepth) put -= kClosed;
     bool ok = true;
     for (; got < put; ++got) ok &= wait_slow(bars + got % kDepth * 8, got / kDepth & 1);
     return ok;

@@ -52,3 +52,19 @@ def test_waits_begin_when_the_predecessor_has_ended(fbmoe_lib, expire, T, N, K):
     y = fbmoe_lib.linear_w4(x, p, N)
     torch.cuda.synchronize()
     check_linear(y, x, v, 64)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_outputs_of_a_failed_layer_are_nan(fbmoe_lib, expire, in_place):
+    """Nothing of what stood in the output, or of what the call got to, is left as if it were a result."""
+    c = Case(fbmoe_lib, 9, 32, 0, 256, 128, 64, 64, BF16, "group", 5)
+    want = fbmoe_lib.forward_w4(*c.args())
+    args = list(c.args())
+    args[2] = c.x.clone()
+    out = args[2] if in_place else torch.full_like(want, 5.0)
+    expire(1)
+    with pytest.raises(fbmoe_lib.DeviceStatusError):
+        fbmoe_lib.forward_w4(*args, out=out, sync_status=True)
+    expire(0)
+    assert out.isnan().all()
+    assert torch.equal(fbmoe_lib.forward_w4(*c.args(), sync_status=True), want)
