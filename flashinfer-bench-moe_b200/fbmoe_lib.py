@@ -596,8 +596,9 @@ def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2
     (``out`` may be hidden_states itself).  Activations are taken as they are, sums are fp32, the SwiGLU output is held as
     two bf16 numbers (within 2^-16 of itself) and the result is rounded once.
     The workspace is allocated per call, so calls may overlap and captured graphs share nothing.  Device-side errors
-    (a bounded wait that expired) raise DeviceStatusError as in ``forward``: at a later call on the device or at
-    check_status(), or for this call with ``sync_status`` (or FBMOE_SYNC_STATUS=1)."""
+    (a bounded wait that expired; the outputs are NaN) raise DeviceStatusError as in ``forward``: at a later call on the
+    device, whichever stream it is on, or at check_status(); with ``sync_status`` (or FBMOE_SYNC_STATUS=1) the call waits
+    for its own status, raises for it and leaves nothing to be reported later."""
     N1, H, group1 = _w4_shape(gemm1_weights, "gemm1_weights")
     N2, I, group2 = _w4_shape(gemm2_weights, "gemm2_weights")
     x, shape1, shape2 = hidden_states, gemm1_weights.shape, gemm2_weights.shape
@@ -631,14 +632,14 @@ def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2
         word = _take_sink(key)
         if word:
             raise DeviceStatusError(word, "reported by an earlier forward_w4 on this device")
+        sync = sync_status_default() if sync_status is None else sync_status
         nbytes = load_library().fbmoe_w4_workspace_size(T, H, I)
         ws = x.new_empty(nbytes, dtype=torch.uint8)
         _launch_on(dev, "fbmoe_forward_w4", routing_logits.data_ptr(), routing_bias.data_ptr(), x.data_ptr(),
                    _W4_X_TYPES[x.dtype], gemm1_weights.data_ptr(), group1, gemm2_weights.data_ptr(), group2, T, H, I, E,
-                   offset, routed_scaling_factor, out.data_ptr(), ws.data_ptr(), nbytes, sink)
-        if sync_status_default() if sync_status is None else sync_status:
-            torch.cuda.current_stream(x.device).synchronize()
-            word = _take_sink(key)
+                   offset, routed_scaling_factor, out.data_ptr(), ws.data_ptr(), nbytes, None if sync else sink)
+        if sync:
+            word = read_status(ws)  # this call's own; the sink is for all of the device's calls
             if word:
                 raise DeviceStatusError(word, "reported by this forward_w4")
     return out

@@ -68,3 +68,56 @@ def test_outputs_of_a_failed_layer_are_nan(fbmoe_lib, expire, in_place):
     expire(0)
     assert out.isnan().all()
     assert torch.equal(fbmoe_lib.forward_w4(*c.args(), sync_status=True), want)
+
+
+def test_a_failed_call_is_reported_once_and_by_itself(fbmoe_lib, expire):
+    """A call that fails on one stream, and one that succeeds after it on another and asks for its own status."""
+    c = Case(fbmoe_lib, 5, 32, 0, 256, 128, 64, 64, BF16, "group", 6)
+    want = fbmoe_lib.forward_w4(*c.args(), sync_status=True)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    expire(1)
+    with torch.cuda.stream(a):
+        fbmoe_lib.forward_w4(*c.args())     # fails 2 ms from now
+    expire(0)
+    with torch.cuda.stream(b):
+        y = fbmoe_lib.forward_w4(*c.args(), sync_status=True)  # its own status is clean
+    assert torch.equal(y, want)
+    with pytest.raises(fbmoe_lib.DeviceStatusError):
+        fbmoe_lib.check_status()
+    fbmoe_lib.check_status()
+    expire(1)
+    with pytest.raises(fbmoe_lib.DeviceStatusError):
+        fbmoe_lib.forward_w4(*c.args(), sync_status=True)
+    expire(0)
+    fbmoe_lib.check_status()                # it has been reported
+
+
+def test_two_threads_get_their_own_status(fbmoe_lib, expire):
+    """Two threads whose calls all fail, each asking for its own status: none takes the other's."""
+    import threading
+    cases = [Case(fbmoe_lib, T, 16, 0, 256, 128, 64, 64, BF16, "group", T) for T in (3, 7)]
+    for c in cases:
+        fbmoe_lib.forward_w4(*c.args(), sync_status=True)
+    torch.cuda.synchronize()
+    seen = [[], []]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(12):
+                try:
+                    fbmoe_lib.forward_w4(*cases[k].args(), sync_status=True)
+                    seen[k].append("none")
+                except fbmoe_lib.DeviceStatusError as e:
+                    seen[k].append("own" if "this forward_w4" in str(e) else "other")
+
+    expire(1)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    expire(0)
+    torch.cuda.synchronize()
+    assert seen == [["own"] * 12] * 2
+    fbmoe_lib.check_status()
