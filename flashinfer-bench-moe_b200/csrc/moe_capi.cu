@@ -504,6 +504,22 @@ int fbmoe_set_status_sink(const void* workspace, uint32_t* sink) {
   return FBMOE_OK;
 }
 
+int fbmoe_alloc_status_word(uint32_t** word) {
+  if (!word) return FBMOE_ERR_NULL_POINTER;
+  // Relaxed for this thread: in the other modes a capture under way, this thread's or another's, refuses allocations.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return from_cuda(e);
+  void* p = nullptr;
+  e = cudaHostAlloc(&p, sizeof(uint32_t), cudaHostAllocPortable);
+  const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e == cudaSuccess) e = back;
+  if (e != cudaSuccess) return from_cuda(e);
+  *static_cast<uint32_t*>(p) = 0;
+  *word = static_cast<uint32_t*>(p);
+  return FBMOE_OK;
+}
+
 int fbmoe_test_expire_grid_wait(int enable) {
   g_test_expire.store(enable == 0 || enable == 2 ? enable : 1, std::memory_order_relaxed);
   return FBMOE_OK;

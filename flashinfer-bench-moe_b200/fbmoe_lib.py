@@ -108,6 +108,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.fbmoe_forward_ep_dispatch.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, f32, i32, i32, vp, vp, u32,
                                                   vp, vp, sz, vp]
         lib.fbmoe_forward_ep_dispatch.restype = i32
+        lib.fbmoe_alloc_status_word.argtypes = [ctypes.POINTER(vp)]
+        lib.fbmoe_alloc_status_word.restype = i32
         i64 = ctypes.c_int64
         lib.fbmoe_w4_bytes.argtypes = [i64, i32, i32, i32]
         lib.fbmoe_w4_bytes.restype = sz
@@ -158,7 +160,7 @@ def block_rows(T: int, E_local: int) -> int:
 # last kernel of every forward stores the call's device status word when it is
 # non-zero (fbmoe_set_status_sink), so errors surface without a host sync.
 _workspaces: Dict[Tuple[int, int], torch.Tensor] = {}
-_sinks: Dict[Tuple[int, int], torch.Tensor] = {}
+_sinks: Dict[Tuple[int, int], object] = {}  # what holds the word: a pinned tensor, or an address (4-bit calls)
 _sink_words: Dict[Tuple[int, int], ctypes.c_uint32] = {}  # the same pinned words, read without torch overhead
 _ws_lock = threading.Lock()
 
@@ -572,20 +574,19 @@ def linear_w4(x: torch.Tensor, weight: torch.Tensor, n: int = None, out: torch.T
 
 
 def _w4_sink(index: int):
-    """(key, address) of the device's status sink for forward_w4: one pinned word that lives as long as the process.  A
-    capture cannot allocate it; a graph captured before the device's first call reports no status."""
+    """(key, address) of the device's status sink for the 4-bit calls: one pinned word, allocated at the first call (which
+    may be a captured one) and there as long as the process."""
     key = (index, -1)
-    sink = _sinks.get(key)
-    if sink is None:
-        if torch.cuda.is_current_stream_capturing():
-            return key, None
+    at = _sinks.get(key)
+    if at is None:
         with _ws_lock:
             if key not in _sinks:
-                sink = torch.zeros(1, dtype=torch.int32).pin_memory()
-                _sink_words[key] = ctypes.c_uint32.from_address(sink.data_ptr())
-                _sinks[key] = sink
-            sink = _sinks[key]
-    return key, sink.data_ptr()
+                word = ctypes.c_void_p()
+                _check(load_library().fbmoe_alloc_status_word(ctypes.byref(word)))
+                _sink_words[key] = ctypes.c_uint32.from_address(word.value)
+                _sinks[key] = word.value
+            at = _sinks[key]
+    return key, at
 
 
 def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2_weights, local_expert_offset,

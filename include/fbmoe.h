@@ -194,6 +194,11 @@ FBMOE_API int fbmoe_read_status(const void* workspace, uint32_t* status, void* s
  * launch and device status (main.py:2062-2070). */
 FBMOE_API int fbmoe_set_status_sink(const void* workspace, uint32_t* sink);
 
+/* *word = a zeroed pinned host word that every device can write: a status sink for
+ * fbmoe_set_status_sink, fbmoe_forward_w4.  May be
+ * called while a stream is being captured.  Free it with cudaFreeHost. */
+FBMOE_API int fbmoe_alloc_status_word(uint32_t** word);
+
 /* How the decode kernel (T <= 64) was last launched: 0 not yet, 1 cooperative
  * with programmatic serialization, 2 cooperative, 3 plain programmatic launch
  * (the default).  Its CTAs wait for one another at a grid-wide arrival: every

@@ -121,3 +121,37 @@ def test_two_threads_get_their_own_status(fbmoe_lib, expire):
     torch.cuda.synchronize()
     assert seen == [["own"] * 12] * 2
     fbmoe_lib.check_status()
+
+
+def test_a_graph_captured_before_the_first_call_reports_its_status():
+    """In a process whose first 4-bit call on the device is a captured one."""
+    import subprocess
+    code = r"""
+import os, sys
+sys.path[:0] = [os.path.join(os.environ["FBMOE_REPO"], "flashinfer-bench-moe_b200"), os.path.join(os.environ["FBMOE_REPO"], "tests")]
+import torch
+import fbmoe_lib as L
+from test_gpu_w4 import Case, BF16, random_packed
+c = Case(L, 4, 32, 0, 256, 128, 64, 64, BF16, "group", 7)
+graphs, outs = [], []
+for mode in (1, 0):
+    L.load_library().fbmoe_test_expire_grid_wait(mode)
+    graphs.append(torch.cuda.CUDAGraph())
+    with torch.cuda.graph(graphs[-1]):
+        outs.append(L.forward_w4(*c.args()))
+graphs[1].replay()
+L.check_status()
+c.check(outs[1])
+graphs[0].replay()
+try:
+    L.check_status()
+    print("silent")
+except L.DeviceStatusError as e:
+    print("word", e.word)
+graphs[1].replay()
+L.check_status()
+c.check(outs[1])
+"""
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, FBMOE_REPO=REPO), capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stderr[-3000:]
+    assert r.stdout.split() == ["word", "4"]
