@@ -166,7 +166,7 @@ template <typename A, int G, int NP>
 __global__ void __launch_bounds__(kRowsThreads, 1)
     rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
                 const __grid_constant__ CUtensorMap map_x, int T, int N, int kt_n,
-                int splits, typename A::Raw* __restrict__ out, long ldo, uint64_t wait_ns) {
+                int splits, typename A::Raw* __restrict__ out, long ldo, uint64_t wait_ns, bool expire, uint32_t* sink) {
   using S = RowsSmem<G, NP>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -177,7 +177,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
            *x_empty = x_full + kXStages, *dec_full = x_empty + kXStages, *dec_empty = dec_full + S::kDecoded,
            *sum_full = dec_empty + S::kDecoded, *sum_empty = sum_full + 8, *scale_full = sum_empty + 8,
            *drain = scale_full + kScaleSlots;
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + kIssuers);
+  uint64_t* never = drain + kIssuers;  // test hook: nothing arrives there
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(never + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_at + 1);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = splits > 1 ? (int)cluster_rank() : 0, unit = blockIdx.x / splits;
@@ -189,6 +190,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     for (int i = 0; i < 8; ++i) mbar_init(&sum_full[i], 1), mbar_init(&sum_empty[i], 4 * kTotals);
     for (int i = 0; i < kScaleSlots; ++i) mbar_init(&scale_full[i], 4);
     for (int i = 0; i < kIssuers; ++i) mbar_init(&drain[i], 1);
+    mbar_init(never, 1);
     *abort = 0;
     fence_barrier_init();
   }
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   pdl_wait();  // every thread: a role's limit counts from here, however long the predecessor takes
   pdl_trigger();
   const uint32_t tmem = *tmem_at;
-  // A wait that gives up raises `abort`, and every role ends; the outputs are then written as NaN.
+  // A wait that gives up raises `abort`, and every role ends; the CTA's outputs are then NaN, and the sink tells.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_wait(bar, parity, abort, wait_ns)) return true;
     *abort = 1;
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   } else if (totals) {
     const int q = warp & 3, row = 32 * q + lane;
     const uint32_t from = tmem + ((uint32_t)(32 * q) << 16) + t_first;
-    bool ok = true;
+    bool ok = !expire || wait_warp(never, 0);
     for (int i = 0; i < steps && ok; ++i) {
       const int ci = i % kScaleSlots;
       ok = wait(&scale_full[ci], i / kScaleSlots & 1);
@@ -402,11 +404,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (threadIdx.x == 0 && sink && *abort) {
+    *reinterpret_cast<volatile uint32_t*>(sink) = kStatusTimeoutEpilogue;
+    __threadfence_system();
+  }
 }
 
 template <typename A, int G, int NP>
 cudaError_t run_rows(const void* x, long ldx, int T, const void* packed, int N, int K, void* out, long ldo,
-                     cudaStream_t stream) {
+                     uint32_t* sink, cudaStream_t stream) {
   using S = RowsSmem<G, NP>;
   static DeviceFlags smem_set;
   cudaError_t e = set_max_dynamic_smem(rows_kernel<A, G, NP>, S::total, smem_set);
@@ -439,7 +445,8 @@ cudaError_t run_rows(const void* x, long ldx, int T, const void* packed, int N, 
   cfg.attrs = attr;
   cfg.numAttrs = splits > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, rows_kernel<A, G, NP>, map_w, map_s, map_x, T, N, kt, splits,
-                            reinterpret_cast<typename A::Raw*>(out), ldo, test_short_waits() ? kTestGridWaitNs : kWaitBudgetNs);
+                            reinterpret_cast<typename A::Raw*>(out), ldo, test_short_waits() ? kTestGridWaitNs : kWaitBudgetNs,
+                            test_expire_grid_wait(), sink);
 }
 
 // Which kernel, by how much there is to spread over the SMs.  tiles_kernel reads the matrix once per 16 tokens and starts and
@@ -463,16 +470,16 @@ bool rows_pay(int T, int N, int K) {
 
 template <typename A, int G>
 cudaError_t run_linear(const void* x, long ldx, int T, const void* packed, int N, int K, void* out, long ldo,
-                       cudaStream_t stream) {
+                       uint32_t* sink, cudaStream_t stream) {
   using Raw = typename A::Raw;
   const unsigned nt = (unsigned)((N - 1) / kTileN + 1);
   const Raw* xp = reinterpret_cast<const Raw*>(x);
   const uint8_t* wp = reinterpret_cast<const uint8_t*>(packed);
   Raw* op = reinterpret_cast<Raw*>(out);
   if (rows_pay(T, N, K)) {
-    if (T <= 16) return run_rows<A, G, 16>(x, ldx, T, packed, N, K, out, ldo, stream);
-    if (T <= 32) return run_rows<A, G, 32>(x, ldx, T, packed, N, K, out, ldo, stream);
-    return run_rows<A, G, 64>(x, ldx, T, packed, N, K, out, ldo, stream);
+    if (T <= 16) return run_rows<A, G, 16>(x, ldx, T, packed, N, K, out, ldo, sink, stream);
+    if (T <= 32) return run_rows<A, G, 32>(x, ldx, T, packed, N, K, out, ldo, sink, stream);
+    return run_rows<A, G, 64>(x, ldx, T, packed, N, K, out, ldo, sink, stream);
   }
   const dim3 grid(nt, (unsigned)((T + 15) / 16)), block(kWarps * 32);
   if (T > 8) return launch_pdl(tiles_kernel<A, G, 2, false>, grid, block, 0, stream, xp, ldx, T, wp, N, K, op, ldo);
@@ -486,10 +493,10 @@ cudaError_t run_linear(const void* x, long ldx, int T, const void* packed, int N
 }
 template <typename A>
 cudaError_t pick_linear(int group, const void* x, long ldx, int T, const void* packed, int N, int K, void* out,
-                        long ldo, cudaStream_t stream) {
-  if (group == 32) return run_linear<A, 32>(x, ldx, T, packed, N, K, out, ldo, stream);
-  if (group == 64) return run_linear<A, 64>(x, ldx, T, packed, N, K, out, ldo, stream);
-  return run_linear<A, 128>(x, ldx, T, packed, N, K, out, ldo, stream);
+                        long ldo, uint32_t* sink, cudaStream_t stream) {
+  if (group == 32) return run_linear<A, 32>(x, ldx, T, packed, N, K, out, ldo, sink, stream);
+  if (group == 64) return run_linear<A, 64>(x, ldx, T, packed, N, K, out, ldo, sink, stream);
+  return run_linear<A, 128>(x, ldx, T, packed, N, K, out, ldo, sink, stream);
 }
 
 }  // namespace
@@ -499,18 +506,25 @@ cudaError_t pick_linear(int group, const void* x, long ldx, int T, const void* p
 using namespace fbmoe;
 
 extern "C" FBMOE_API int fbmoe_linear_w4(const void* x, int64_t x_stride, int type, int T, const void* packed, int N,
-                                         int K, int group, void* out, int64_t out_stride, void* stream_) {
+                                         int K, int group, void* out, int64_t out_stride, void* stream) {
+  return fbmoe_linear_w4_status(x, x_stride, type, T, packed, N, K, group, out, out_stride, nullptr, stream);
+}
+
+extern "C" FBMOE_API int fbmoe_linear_w4_status(const void* x, int64_t x_stride, int type, int T, const void* packed,
+                                                int N, int K, int group, void* out, int64_t out_stride,
+                                                uint32_t* status_sink, void* stream_) {
   if (T < 0 || T > w4::kMaxTokens || N < 1 || K < 128 || K % 128 != 0 || !w4::valid_group(group) ||
       (type != FBMOE_BF16 && type != FBMOE_F16) || x_stride < K || out_stride < N)
     return FBMOE_ERR_INVALID_ARG;
   if (T == 0) return FBMOE_OK;
   if (!x || !packed || !out) return FBMOE_ERR_NULL_POINTER;
-  if (((uintptr_t)x & 15) || (x_stride & 7) || ((uintptr_t)packed & 15) || ((uintptr_t)out & 1))
+  if (((uintptr_t)x & 15) || (x_stride & 7) || ((uintptr_t)packed & 15) || ((uintptr_t)out & 1) ||
+      ((uintptr_t)status_sink & 3))
     return FBMOE_ERR_MISALIGNED;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const cudaError_t e =
       type == FBMOE_BF16
-          ? w4::pick_linear<w4::Bf16>(group, x, x_stride, T, packed, N, K, out, out_stride, stream)
-          : w4::pick_linear<w4::F16>(group, x, x_stride, T, packed, N, K, out, out_stride, stream);
+          ? w4::pick_linear<w4::Bf16>(group, x, x_stride, T, packed, N, K, out, out_stride, status_sink, stream)
+          : w4::pick_linear<w4::F16>(group, x, x_stride, T, packed, N, K, out, out_stride, status_sink, stream);
   return e == cudaSuccess ? FBMOE_OK : (int)e;
 }

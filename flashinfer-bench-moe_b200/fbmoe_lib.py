@@ -119,6 +119,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.fbmoe_dequantize_w4.restype = i32
         lib.fbmoe_linear_w4.argtypes = [vp, i64, i32, i32, vp, i32, i32, i32, vp, i64, vp]
         lib.fbmoe_linear_w4.restype = i32
+        lib.fbmoe_linear_w4_status.argtypes = [vp, i64, i32, i32, vp, i32, i32, i32, vp, i64, vp, vp]
+        lib.fbmoe_linear_w4_status.restype = i32
         lib.fbmoe_w4_workspace_size.argtypes = [i32, i32, i32]
         lib.fbmoe_w4_workspace_size.restype = sz
         lib.fbmoe_forward_w4.argtypes = [vp, vp, vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, vp, vp, sz,
@@ -543,7 +545,9 @@ def dequantize_w4(packed: torch.Tensor, n: int = None, dtype: torch.dtype = torc
 def linear_w4(x: torch.Tensor, weight: torch.Tensor, n: int = None, out: torch.Tensor = None) -> torch.Tensor:
     """``x @ W^T`` for at most 64 tokens: x [T, K] bfloat16 or float16 (rows may be strided by a multiple of 8
     elements), ``weight`` one packed [n, K] matrix; returns [T, n] in x's type, summed in fp32; ``out`` must not
-    overlap x.  More tokens: a GEMM on ``dequantize_w4(weight, n)``."""
+    overlap x.  A bounded wait that expired (calls of more than 8 tokens have such waits) makes the outputs NaN and raises
+    DeviceStatusError at a later such call on the device or at check_status().  More tokens: a GEMM on
+    ``dequantize_w4(weight, n)``."""
     n, K, group = _w4_shape(weight, "weight", n)
     _require(weight.dim() == 3, "weight must be one packed matrix [ceil(N / 16), K / 128, tile]")
     _require(isinstance(x, torch.Tensor) and x.dtype in _W4_X_TYPES, "x must be bfloat16 or float16")
@@ -567,15 +571,18 @@ def linear_w4(x: torch.Tensor, weight: torch.Tensor, n: int = None, out: torch.T
                  and out.stride(1) == 1 and (T <= 1 or out.stride(0) >= n),
                  "out must be [T, n] in x's type on x's device, its rows contiguous")
         out_stride = out.stride(0) if T > 1 else n
-    if T:
+    if T > 8:
+        _launch_on(dev, "fbmoe_linear_w4_status", x.data_ptr(), x_stride, _W4_X_TYPES[x.dtype], T, weight.data_ptr(), n, K,
+                   group, out.data_ptr(), out_stride, _w4_sink(dev))
+    elif T:
         _launch_on(dev, "fbmoe_linear_w4", x.data_ptr(), x_stride, _W4_X_TYPES[x.dtype], T, weight.data_ptr(), n, K,
                    group, out.data_ptr(), out_stride)
     return out
 
 
-def _w4_sink(index: int):
-    """(key, address) of the device's status sink for the 4-bit calls: one pinned word, allocated at the first call (which
-    may be a captured one) and there as long as the process."""
+def _w4_sink(index: int) -> int:
+    """The address of the device's status sink for the 4-bit calls: one pinned word, allocated at the first call (which may
+    be a captured one) and there as long as the process.  Raises what an earlier call left there."""
     key = (index, -1)
     at = _sinks.get(key)
     if at is None:
@@ -586,7 +593,10 @@ def _w4_sink(index: int):
                 _sink_words[key] = ctypes.c_uint32.from_address(word.value)
                 _sinks[key] = word.value
             at = _sinks[key]
-    return key, at
+    word = _take_sink(key)
+    if word:
+        raise DeviceStatusError(word, "reported by an earlier 4-bit call on this device")
+    return at
 
 
 def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2_weights, local_expert_offset,
@@ -629,10 +639,7 @@ def forward_w4(routing_logits, routing_bias, hidden_states, gemm1_weights, gemm2
         _require(out.dtype == x.dtype and out.shape == (T, H) and out.is_contiguous() and out.get_device() == dev,
                  "out must be contiguous [T, H] in hidden_states' type on its device")
     if T:
-        key, sink = _w4_sink(dev)
-        word = _take_sink(key)
-        if word:
-            raise DeviceStatusError(word, "reported by an earlier forward_w4 on this device")
+        sink = _w4_sink(dev)
         sync = sync_status_default() if sync_status is None else sync_status
         nbytes = load_library().fbmoe_w4_workspace_size(T, H, I)
         ws = x.new_empty(nbytes, dtype=torch.uint8)

@@ -195,7 +195,7 @@ FBMOE_API int fbmoe_read_status(const void* workspace, uint32_t* status, void* s
 FBMOE_API int fbmoe_set_status_sink(const void* workspace, uint32_t* sink);
 
 /* *word = a zeroed pinned host word that every device can write: a status sink for
- * fbmoe_set_status_sink, fbmoe_forward_w4.  May be
+ * fbmoe_set_status_sink, fbmoe_forward_w4 and fbmoe_linear_w4_status.  May be
  * called while a stream is being captured.  Free it with cudaFreeHost. */
 FBMOE_API int fbmoe_alloc_status_word(uint32_t** word);
 
@@ -212,6 +212,7 @@ FBMOE_API int fbmoe_decode_launch_mode(void);
  * waits for one arrival that never comes, with a 2 ms budget, so every CTA's
  * bounded wait expires, sets status bit 2 and returns without writing its part
  * of the output.  Lets tests exercise the error path without any device fault.
+ * So do waits of fbmoe_forward_w4 and fbmoe_linear_w4, whose outputs become NaN.
  * 2: nothing is missing, and the waits of fbmoe_linear_w4 have that budget. */
 FBMOE_API int fbmoe_test_expire_grid_wait(int enable);
 
@@ -336,9 +337,13 @@ FBMOE_API int fbmoe_dequantize_w4(const void* packed, int64_t batch, int N, int 
 /* out[t, n] = sum over k of x[t, k] * w[n, k] for 0 <= T <= 64 tokens: x and out of
  * `type` (FBMOE_BF16 or FBMOE_F16), rows x_stride and out_stride elements apart
  * (x 16-byte aligned, x_stride a multiple of 8; out overlaps neither x nor packed),
- * sums in fp32.  A bounded wait that expires makes outputs NaN. */
+ * sums in fp32.  A bounded wait that expires (calls of more than 8 tokens have such
+ * waits) makes outputs NaN; fbmoe_linear_w4_status also stores a status word (the bits
+ * of fbmoe_read_status) to status_sink, as fbmoe_forward_w4 does. */
 FBMOE_API int fbmoe_linear_w4(const void* x, int64_t x_stride, int type, int T, const void* packed, int N, int K,
                               int group, void* out, int64_t out_stride, void* stream);
+FBMOE_API int fbmoe_linear_w4_status(const void* x, int64_t x_stride, int type, int T, const void* packed, int N, int K,
+                                     int group, void* out, int64_t out_stride, uint32_t* status_sink, void* stream);
 
 /* The fused MoE layer on packed 4-bit weights for 0 <= T <= 64 tokens: routing as
  * fbmoe_forward (256 experts, top-8), hidden_states and out [T, H] of `type`

@@ -155,3 +155,46 @@ c.check(outs[1])
     r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, FBMOE_REPO=REPO), capture_output=True, text=True, timeout=600)
     assert r.returncode == 0, r.stderr[-3000:]
     assert r.stdout.split() == ["word", "4"]
+
+
+@pytest.mark.parametrize("T,N,K", [(16, 130, 12288), (64, 18432, 1024)])  # clusters, single CTAs
+def test_a_failed_linear_is_nan_and_reported(fbmoe_lib, expire, T, N, K):
+    p, v = random_packed(N, K, 64, 3)
+    x = torch.randn((T, K), generator=torch.Generator().manual_seed(4)).to(BF16).cuda()
+    want = fbmoe_lib.linear_w4(x, p, N)
+    expire(1)
+    out = torch.full((T + 1, N + 8), 7.0, dtype=BF16, device="cuda")
+    fbmoe_lib.linear_w4(x, p, N, out=out[:T, 4:N + 4])
+    expire(0)
+    with pytest.raises(fbmoe_lib.DeviceStatusError) as e:
+        fbmoe_lib.check_status()
+    assert e.value.word & 4
+    assert out[:T, 4:N + 4].isnan().all()
+    assert (out[:, :4] == 7).all() and (out[:, N + 4:] == 7).all() and (out[T] == 7).all()
+    assert torch.equal(fbmoe_lib.linear_w4(x, p, N), want)
+    fbmoe_lib.check_status()
+    expire(1)
+    fbmoe_lib.linear_w4(x, p, N)
+    expire(0)
+    torch.cuda.synchronize()
+    with pytest.raises(fbmoe_lib.DeviceStatusError):
+        fbmoe_lib.linear_w4(x, p, N)        # the next call says so
+    assert torch.equal(fbmoe_lib.linear_w4(x, p, N), want)
+    fbmoe_lib.check_status()
+
+
+def test_a_captured_linear_reports_its_status(fbmoe_lib, expire):
+    p, _ = random_packed(130, 12288, 64, 3)
+    x = torch.randn((12, 12288), generator=torch.Generator().manual_seed(4)).to(BF16).cuda()
+    want = fbmoe_lib.linear_w4(x, p, 130)
+    expire(1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fbmoe_lib.linear_w4(x, p, 130)
+    expire(0)
+    for _ in range(2):
+        graph.replay()
+        with pytest.raises(fbmoe_lib.DeviceStatusError):
+            fbmoe_lib.check_status()
+        assert y.isnan().all()
+    assert torch.equal(fbmoe_lib.linear_w4(x, p, 130), want)
