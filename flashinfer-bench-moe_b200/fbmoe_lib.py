@@ -462,6 +462,7 @@ _W4_GROUPS = {1024 + 4096 // g: g for g in (32, 64, 128)}
 _W4_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
 _W4_X_TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _fns: Dict[str, object] = {}  # C entry points by name
+_INT_MAX = 0x7FFFFFFF
 
 
 def _launch_on(index: int, name: str, *args) -> None:
@@ -490,7 +491,10 @@ def _w4_shape(packed: torch.Tensor, name: str, n: int = None) -> Tuple[int, int,
         n = rows
     elif not rows - 16 < n <= rows:
         raise RuntimeError(f"n must be in {rows - 15}..{rows} for {name}'s {shape[-3]} row tiles")
-    return int(n), shape[-2] * 128, _W4_GROUPS[shape[-1]]
+    K = shape[-2] * 128
+    if n > _INT_MAX or K > _INT_MAX:  # the C ABI's sizes have 32 bits
+        raise RuntimeError(f"{name}'s N and K must be below 2^31")
+    return int(n), K, _W4_GROUPS[shape[-1]]
 
 
 def quantize_w4(w: torch.Tensor, group_size: int = 128, scale: torch.Tensor = None,
@@ -508,6 +512,7 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, scale: torch.Tensor = No
     shape = tuple(w.shape)
     lead, N, K = shape[:-2], shape[-2], shape[-1]
     _require(N > 0 and K > 0 and K % 128 == 0, "K must be a positive multiple of 128 and N positive")
+    _require(N <= _INT_MAX and K <= _INT_MAX, "N and K must be below 2^31")
     _require((block_scale is not None) == (w.dtype == torch.float8_e4m3fn),
              "block_scale goes with float8_e4m3fn weights, and only with them")
     if block_scale is not None:

@@ -131,3 +131,24 @@ def test_c_entry_points_refuse(fbmoe_lib):
     for bad in (dict(T=65), dict(T=-1), dict(H=64), dict(I=200), dict(E=0), dict(E=257), dict(off=-1), dict(off=256),
                 dict(type_=2), dict(g1=16), dict(g2=256), dict(H=1 << 21)):
         assert m(**bad) == -1, bad
+
+
+def test_sizes_past_32_bits_are_refused(fbmoe_lib):
+    """N and K are 32-bit numbers in the C ABI: larger ones are refused, not cut to their low half.  (Shapes only: tensors
+    without memory.)"""
+    L, big = fbmoe_lib, 1 << 32
+    meta = dict(device="meta")
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        L.dequantize_w4(torch.empty((1, big // 128 + 1, 1056), dtype=torch.uint8, **meta), 1)  # K = 2^32 + 128
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        L.dequantize_w4(torch.empty((big // 16 + 1, 1, 1056), dtype=torch.uint8, **meta))
+    for shape in ((1, big + 128), (big + 1, 128), (1 << 31, 128)):
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            L.quantize_w4(torch.empty(shape, dtype=torch.bfloat16, **meta))
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        L.linear_w4(torch.empty((1, big + 128), dtype=torch.bfloat16, **meta),
+                    torch.empty((1, big // 128 + 1, 1056), dtype=torch.uint8, **meta))
+    with pytest.raises(RuntimeError, match="CUDA"):  # the largest of either
+        L.dequantize_w4(torch.empty((1, (1 << 24) - 1, 1056), dtype=torch.uint8, **meta))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        L.dequantize_w4(torch.empty((1 << 27, 1, 1056), dtype=torch.uint8, **meta), (1 << 31) - 1)
