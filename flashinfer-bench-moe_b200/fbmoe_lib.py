@@ -547,10 +547,23 @@ def dequantize_w4(packed: torch.Tensor, n: int = None, dtype: torch.dtype = torc
     return out
 
 
+def _rows_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether rows of a and of b [rows, width], contiguous and of one element size, share memory.  Rows that lie in each
+    other's gaps are told apart where both are the same distance apart, and otherwise taken to meet."""
+    size = a.element_size()
+    a0, b0, wa, wb = a.data_ptr(), b.data_ptr(), a.size(1) * size, b.size(1) * size
+    sa = a.stride(0) * size if a.size(0) > 1 else max(wa, b.stride(0) * size)
+    sb = b.stride(0) * size if b.size(0) > 1 else max(wb, sa)
+    if b0 >= a0 + sa * (a.size(0) - 1) + wa or a0 >= b0 + sb * (b.size(0) - 1) + wb:
+        return False
+    at = (b0 - a0) % sa
+    return sa != sb or at < wa or at + wb > sa
+
+
 def linear_w4(x: torch.Tensor, weight: torch.Tensor, n: int = None, out: torch.Tensor = None) -> torch.Tensor:
     """``x @ W^T`` for at most 64 tokens: x [T, K] bfloat16 or float16 (rows may be strided by a multiple of 8
     elements), ``weight`` one packed [n, K] matrix; returns [T, n] in x's type, summed in fp32; ``out`` must not
-    overlap x.  A bounded wait that expired (calls of more than 8 tokens have such waits) makes the outputs NaN and raises
+    overlap x or weight (columns of one tensor beside each other do not).  A bounded wait that expired (calls of more than 8 tokens have such waits) makes the outputs NaN and raises
     DeviceStatusError at a later such call on the device or at check_status().  More tokens: a GEMM on
     ``dequantize_w4(weight, n)``."""
     n, K, group = _w4_shape(weight, "weight", n)
@@ -575,6 +588,8 @@ def linear_w4(x: torch.Tensor, weight: torch.Tensor, n: int = None, out: torch.T
         _require(out.dtype == x.dtype and tuple(out.shape) == (T, n) and out.get_device() == dev
                  and out.stride(1) == 1 and (T <= 1 or out.stride(0) >= n),
                  "out must be [T, n] in x's type on x's device, its rows contiguous")
+        _require(not T or not (_rows_meet(x, out) or _rows_meet(weight.view(x.dtype).view(1, -1), out)),
+                 "out must not overlap x or weight")
         out_stride = out.stride(0) if T > 1 else n
     if T > 8:
         _launch_on(dev, "fbmoe_linear_w4_status", x.data_ptr(), x_stride, _W4_X_TYPES[x.dtype], T, weight.data_ptr(), n, K,

@@ -152,3 +152,24 @@ def test_sizes_past_32_bits_are_refused(fbmoe_lib):
         L.dequantize_w4(torch.empty((1, (1 << 24) - 1, 1056), dtype=torch.uint8, **meta))
     with pytest.raises(RuntimeError, match="CUDA"):
         L.dequantize_w4(torch.empty((1 << 27, 1, 1056), dtype=torch.uint8, **meta), (1 << 31) - 1)
+
+
+@pytest.mark.parametrize("rows,other", [(1, 1), (1, 4), (4, 4), (4, 9), (3, 1)])
+def test_rows_that_share_memory_are_found(fbmoe_lib, rows, other):
+    """Against the sets of elements, for two windows of one buffer at all offsets."""
+    def elements(t):
+        return {t.storage_offset() + r * t.stride(0) + c for r in range(t.size(0)) for c in range(t.size(1))}
+
+    buf = torch.zeros(400, dtype=torch.float16)
+    for wide, narrow in ((10, 10), (12, 5), (7, 3)):
+        a = buf.as_strided((rows, narrow), (wide, 1), 100)
+        for at in range(0, 260):
+            for stride, width in ((wide, wide - narrow), (wide, 1), (8, 8)):
+                b = buf.as_strided((other, max(width, 1)), (stride, 1), at)
+                meet = bool(elements(a) & elements(b))
+                found = fbmoe_lib._rows_meet(a, b)
+                assert found or not meet
+                if stride == wide or rows == other == 1:
+                    # the same distance apart: exact, but for windows whose columns meet in rows past one another's last
+                    columns = {i % wide for i in elements(a)} & {i % wide for i in elements(b)}
+                    assert not found or meet or columns
