@@ -210,19 +210,21 @@ __global__ void __launch_bounds__(kWarps * 32, TYPE == kF32 ? 2 : 4) quantize_ke
     if (t == 0) *reinterpret_cast<uint32_t*>(out + kTileQ + 32 * gr + 4 * g) = scale_word[gr];
 }
 
-// Eight consecutive values in the output type.
+// Eight consecutive values in the output type, stored where `there`; called by all lanes of a warp.
 template <int TYPE>
-__device__ __forceinline__ void store8(void* base, size_t at, const float (&v)[8]) {
+__device__ __forceinline__ void store8(void* base, size_t at, const float (&v)[8], bool there) {
   if constexpr (TYPE == kF32) {
     // Two lanes of a quad swap halves, so that a store writes whole 32-byte sectors: first the even lane's, then the odd's.
     const bool odd = threadIdx.x & 1;
     float o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __shfl_xor_sync(__activemask(), odd ? v[i] : v[4 + i], 1);
+    for (int i = 0; i < 4; ++i) o[i] = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[4 + i], 1);
+    if (!there) return;
     float* p = reinterpret_cast<float*>(base) + at - (odd ? 4 : 0);
     *reinterpret_cast<float4*>(p) = odd ? make_float4(o[0], o[1], o[2], o[3]) : make_float4(v[0], v[1], v[2], v[3]);
     *reinterpret_cast<float4*>(p + 8) = odd ? make_float4(v[4], v[5], v[6], v[7]) : make_float4(o[0], o[1], o[2], o[3]);
   } else {
+    if (!there) return;
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -257,7 +259,6 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* 
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int row = nt * kTileN + 8 * h + g;
-    if (row >= N) continue;
     const size_t at = ((size_t)b * N + row) * K + (size_t)kt * kTileK + 8 * t;
     const uint32_t w[4] = {q[h].x, q[h].y, q[h].z, q[h].w};
 #pragma unroll
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* 
         v[2 * i] = __uint_as_float(p[i] << 16) * s;
         v[2 * i + 1] = __uint_as_float(p[i] & 0xFFFF0000u) * s;
       }
-      store8<TYPE>(out, at + 32 * j, v);
+      store8<TYPE>(out, at + 32 * j, v, row < N);
     }
   }
   }
