@@ -31,12 +31,13 @@ namespace {
 
 constexpr int kWarps = 8;
 
-// STREAM: the values take no place in the L1 cache, so that x stays there.
+// STREAM: the values take no place in the L1 cache, so that x stays there.  Volatile: not before pdl_wait, the kernel before
+// may have written them.
 template <bool STREAM>
 __device__ __forceinline__ uint4 load_values(const uint8_t* p) {
   if (!STREAM) return __ldg(reinterpret_cast<const uint4*>(p));
   uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 

@@ -408,6 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) layer_kernel(const __grid_constan
   }
   fence_barrier_init();
   pdl_wait();
+  fence_proxy_async_global();  // the weights, read by tensor copies, may be a kernel's of this stream
   pdl_trigger();
   build_lists(a, s);  // synchronises the CTA
   if (threadIdx.x < 2) {
