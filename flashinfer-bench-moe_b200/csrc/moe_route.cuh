@@ -1,6 +1,6 @@
 // moe_route.cuh -- device code of the DeepSeek-V3 no-aux router: route_token()
 // routes one token with one warp, so any kernel can embed the router (the
-// router kernel in moe_route.cu is its only caller today).  The algorithm and
+// router kernel in moe_route.cu and the 4-bit layer's do).  The algorithm and
 // its exactness argument are described in moe_route.cu.
 #pragma once
 #include <float.h>
