@@ -505,7 +505,8 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, scale: torch.Tensor = No
     ``w``: bfloat16, float16 or float32, or float8_e4m3fn with the operator's 128x128 ``block_scale``
     (fp32 [..., ceil(N / 128), K / 128]).  ``scale`` (bf16 [..., N, K / group_size], positive) gives the scales instead,
     so that weights which already are q * scale are packed exactly.  A group holding a NaN or an infinity gets the
-    scale NaN; one whose scale is zero or below the smallest normal number gets zeros."""
+    scale NaN; one whose scale is zero or below the smallest normal number gets zeros, and so does one whose given scale is
+    negative, infinite or NaN (kept as it is: the last two read back as NaN)."""
     _require(isinstance(w, torch.Tensor) and w.dtype in _W4_TYPES, "w must be bfloat16, float16, float32 or float8_e4m3fn")
     _require(w.dim() >= 2 and w.is_contiguous(), "w must be contiguous [..., N, K]")
     _require(group_size in (32, 64, 128), "group_size must be 32, 64 or 128")

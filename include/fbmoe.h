@@ -323,7 +323,8 @@ FBMOE_API size_t fbmoe_w4_bytes(int64_t batch, int N, int K, int group);
  * bf16(max |w| / 7), 0 when that is below the smallest normal number;
  * q = clamp(rint(w / scale), -8, 7) with the IEEE fp32 quotient.  scale_bf16
  * [batch, N, K / group] gives the scales instead (weights that already are
- * q * scale come back exactly); where it is not a positive normal number q is 0.
+ * q * scale come back exactly); where it is not a positive normal number it is kept
+ * and q is 0, which reads back as 0, or as NaN for a scale of infinity or NaN.
  * A group that holds a NaN or an infinity gets the scale NaN.  FBMOE_E4M3 weights
  * are multiplied by block_scale [batch, ceil(N / 128), K / 128] (the operator's own
  * 128x128 scales).  w and packed 16-byte aligned. */

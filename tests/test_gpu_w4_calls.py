@@ -8,7 +8,9 @@ import torch
 from conftest import REPO
 
 sys.path.insert(0, os.path.join(REPO, "tests"))
-from test_gpu_w4 import BF16, F16, check_linear, random_packed  # noqa: E402
+import w4_oracle as W  # noqa: E402
+from test_gpu_w4 import BF16, F16, F32, check_linear, random_packed  # noqa: E402
+from test_gpu_w4_magnitudes import Layer  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +74,81 @@ def test_weights_written_by_the_call_before(fbmoe_lib):
     for r in range(20):
         for y, z in zip(step(r % 2, False), want[r % 2]):
             assert torch.equal(y, z)
+
+
+# ------------------------------------------------------------------ values that are not ordinary numbers
+def test_given_scales_that_are_no_scales(fbmoe_lib):
+    """Kept, with zeros: they read back as 0, or as NaN where the scale is infinite or NaN."""
+    N, G = 16, 64
+    w = torch.randn((N, 128), generator=torch.Generator().manual_seed(1)).cuda()
+    s = torch.ones((N, 2), dtype=BF16)
+    odd = [float("inf"), float("-inf"), float("nan"), 0.0, -0.0, -1.0, 2.0 ** -130, 2.0 ** -126]
+    s[:len(odd), 0] = torch.tensor(odd).to(BF16)
+    p = fbmoe_lib.quantize_w4(w, G, scale=s.cuda())
+    q, s2 = W.unpack(p, N, 128, G)
+    assert torch.equal(s2.view(torch.int16), s.view(torch.int16))
+    assert not q[:7, :G].any() and (q[7, :G].abs() >= 7).all()  # the smallest normal scale is one
+    back = fbmoe_lib.dequantize_w4(p, dtype=F32).cpu()
+    assert back[:3, :G].isnan().all() and (back[3:7, :G] == 0).all()
+    assert torch.equal(back[8:], W.values(p, N, 128, G)[8:].float())
+    assert torch.equal(back[:, G:], W.values(p, N, 128, G)[:, G:].float())
+
+
+class Local:
+    """Local experts' matrices in 64 bits, as w4_oracle.moe takes them."""
+
+    def __init__(self, packed, N, K, G):
+        self.local, self.at = range(packed.shape[0]), lambda e: W.values(packed[e], N, K, G)
+
+    def __call__(self, e):
+        return self.at(e)
+
+
+def bad_token_case(dtype):
+    g = torch.Generator().manual_seed(4)
+    T, E, H, I, G1, G2 = 12, 256, 256, 128, 32, 64
+    logits, bias = torch.randn((T, 256), generator=g).cuda(), (torch.randn(256, generator=g) * 0.1).to(BF16).cuda()
+    x = torch.randn((T, H), generator=g).to(dtype).cuda()
+    w1, w2 = random_packed(2 * I, H, G1, 5, (E,))[0], random_packed(H, I, G2, 6, (E,))[0]
+    return logits, bias, x, w1, w2, Local(w1, 2 * I, H, G1), Local(w2, H, I, G2), I
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_bad_activations_spoil_their_token(fbmoe_lib, dtype, value):
+    """A NaN or an infinity among a token's activations: the formula gives it no finite output (an infinity times each of a
+    row's weights, some of them zero), and the other tokens keep their bits."""
+    logits, bias, x, w1, w2, v1, v2, I = bad_token_case(dtype)
+    clean = fbmoe_lib.forward_w4(logits, bias, x, w1, w2, 0, 2.5)
+    bad = x.clone()
+    bad[5, 2] = value
+    y = fbmoe_lib.forward_w4(logits, bias, bad, w1, w2, 0, 2.5)
+    idx, w = fbmoe_lib.route(logits, bias, 2.5)
+    ref, _ = W.moe(idx[5:6], w[5:6], bad[5:6], v1, v2, 0, I)
+    assert not ref.isfinite().any() and not y[5].isfinite().any()
+    keep = [t for t in range(12) if t != 5]
+    assert torch.equal(y[keep], clean[keep])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_bad_logits(fbmoe_lib, dtype):
+    """What routing gives for logits that are not numbers, carried through the layer: a NaN weight makes its token NaN, a
+    token whose scores are all 0 gets weights of 0 / 1e-20 and zeros."""
+    logits, bias, x, w1, w2, v1, v2, I = bad_token_case(dtype)
+    logits[7] = float("nan")
+    logits[9] = float("-inf")
+    logits[2, :200] = float("-inf")
+    logits[3, 17] = float("inf")
+    y = fbmoe_lib.forward_w4(logits, bias, x, w1, w2, 0, 2.5)
+    idx, w = fbmoe_lib.route(logits, bias, 2.5)
+    assert w[7].isnan().all() and not w[9].any() and w[[2, 3]].isfinite().all()
+    assert y[7].isnan().all() and not y[9].any()
+    good = [t for t in range(12) if t != 7]
+    c = Layer.__new__(Layer)
+    c.T, c.E, c.H, c.I, c.G1, c.G2, c.x, c.idx, c.w = 11, 256, 256, I, 32, 64, x[good], idx[good], w[good]
+    c.v1, c.v2 = [v1(e).cuda() for e in range(256)], [v2(e).cuda() for e in range(256)]
+    assert c.worst(y[good]) <= 1
+    for value in (float("nan"), float("-inf")):
+        logits[:] = value
+        y = fbmoe_lib.forward_w4(logits, bias, x, w1, w2, 0, 2.5)
+        assert y.isnan().all() if value != value else not y.any()
