@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kWarps * 32, TYPE == kF32 ? 2 : 4) quantize_ke
                                                                int K, uint8_t* __restrict__ packed) {
   constexpr int kGroups = 128 / G, kPer = G / 32;  // groups of a tile; words of a lane per group
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t kt_n = K / kTileK, nt_n = (N - 1) / kTileN + 1;
+  const uint32_t kt_n = K / kTileK, nt_n = ((uint32_t)N + kTileN - 1) / kTileN;
   pdl_wait();
   pdl_trigger();
   const uint32_t tile = blockIdx.x * kWarps + (threadIdx.x >> 5);
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kWarps * 32, TYPE == kF32 ? 2 : 4) quantize_ke
     }
   }
   // a tile lies inside one 128 x 128 block
-  const float bs = TYPE == kE4m3 ? __ldg(block_scale + ((size_t)b * ((N - 1) / 128 + 1) + nt / 8) * kt_n + kt) : 1.0f;
+  const float bs = TYPE == kE4m3 ? __ldg(block_scale + ((size_t)b * (((uint32_t)N + 127) / 128) + nt / 8) * kt_n + kt) : 1.0f;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int row = nt * kTileN + 8 * h + g;
@@ -244,7 +244,7 @@ template <int TYPE, int G>
 __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* __restrict__ packed, uint32_t tiles, int N,
                                                                  int K, void* __restrict__ out) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t kt_n = K / kTileK, nt_n = (N - 1) / kTileN + 1;
+  const uint32_t kt_n = K / kTileK, nt_n = ((uint32_t)N + kTileN - 1) / kTileN;
   pdl_wait();
   pdl_trigger();
   for (uint32_t tile = blockIdx.x * kWarps + (threadIdx.x >> 5); tile < tiles; tile += gridDim.x * kWarps) {
