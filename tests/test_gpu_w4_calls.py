@@ -152,3 +152,52 @@ def test_bad_logits(fbmoe_lib, dtype):
         logits[:] = value
         y = fbmoe_lib.forward_w4(logits, bias, x, w1, w2, 0, 2.5)
         assert y.isnan().all() if value != value else not y.any()
+
+
+def test_a_decoder_in_the_same_buffers(fbmoe_lib):
+    """Projection, layer, projection, each reading what the one before wrote, call after call into the same memory with
+    nothing between: every pass gives what it gives alone."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    H, I, T = 1024, 256, 24
+    up, down = random_packed(H, 2048, 64, 1)[0], random_packed(2048, H, 32, 2)[0]
+    w1, w2 = random_packed(2 * I, H, 128, 3, (8,))[0], random_packed(H, I, 64, 4, (8,))[0]
+    inputs = [torch.randn((T, 2048), generator=g, device="cuda").to(BF16) for _ in range(5)]
+    logits = torch.randn((T, 256), generator=g, device="cuda")
+    logits[:, :8] += 4.0
+    bias = torch.zeros(256, dtype=BF16, device="cuda")
+
+    def run(x, t, h, y):
+        fbmoe_lib.linear_w4(x[:t], up, out=h[:t])
+        fbmoe_lib.forward_w4(logits[:t], bias, h[:t], w1, w2, 0, 2.5, out=h[:t])
+        fbmoe_lib.linear_w4(h[:t], down, out=y[:t])
+
+    want = {}
+    for i, x in enumerate(inputs):
+        for t in (1, 8, T):
+            h, y = torch.empty((T, H), dtype=BF16, device="cuda"), torch.empty((T, 2048), dtype=BF16, device="cuda")
+            run(x, t, h, y)
+            torch.cuda.synchronize()
+            want[i, t] = y[:t].clone()
+    h, y = torch.empty((T, H), dtype=BF16, device="cuda"), torch.empty((T, 2048), dtype=BF16, device="cuda")
+    got = []
+    for r in range(60):
+        i, t = r % 5, (1, 8, T)[r % 3]
+        run(inputs[i], t, h, y)
+        got.append((i, t, y[:t].clone()) if r % 2 else None)
+    torch.cuda.synchronize()
+    assert all(torch.equal(z, want[i, t]) for i, t, z in filter(None, got))
+    x = inputs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):  # three layers of the same weights
+            run(x, T, h, y)
+            x.copy_(y)
+    ref = inputs[1].clone()
+    for _ in range(3):
+        run(ref, T, h, y)
+        torch.cuda.synchronize()
+        ref = y.clone()
+    for _ in range(4):
+        x.copy_(inputs[1])
+        graph.replay()
+        assert torch.equal(x, ref)
