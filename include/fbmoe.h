@@ -351,11 +351,12 @@ FBMOE_API int fbmoe_linear_w4_status(const void* x, int64_t x_stride, int type, 
  * (FBMOE_BF16 or FBMOE_F16), gemm1_weights E_local packed [2I, H] matrices (rows
  * [0, I) the linear half, [I, 2I) the silu half), gemm2_weights E_local packed
  * [H, I] matrices; H and I multiples of 128; sums in fp32, the intermediate held
- * as two bf16 numbers (within 2^-16 of itself), the result rounded once.  Pointers 16-byte aligned; workspace >= fbmoe_w4_workspace_size(T, H, I)
+ * as two bf16 numbers (within 2^-16 of itself), the result rounded once.  out may be
+ * hidden_states.  Pointers 16-byte aligned; workspace >= fbmoe_w4_workspace_size(T, H, I)
  * bytes, 256-byte aligned; calls that may overlap need a workspace each.  A bounded
  * wait that expires makes outputs NaN, sets the status word at the workspace's start
- * (the bits of fbmoe_read_status) and stores it to status_sink (device-accessible, e.g. pinned host memory;
- * sticky; may be NULL). */
+ * (the bits of fbmoe_read_status) and stores it to status_sink (device-accessible, e.g.
+ * pinned host memory; sticky; may be NULL). */
 FBMOE_API size_t fbmoe_w4_workspace_size(int T, int H, int I);
 FBMOE_API int fbmoe_forward_w4(const float* routing_logits, const void* routing_bias, const void* hidden_states,
                                int type, const void* gemm1_weights, int group1, const void* gemm2_weights, int group2,
